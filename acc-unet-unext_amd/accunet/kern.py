@@ -587,3 +587,56 @@ def relu(x, dy, y):
 
 def subsample2(src, dst, B, H, W, C, bwd):
     call("accunet_subsample2", _p(src), _p(dst), B, H, W, C, int(bwd), _stream())
+
+
+# --------------------------------------------------- norms around a residual block
+def blocknorm_fwd(x, f, w1, b1, s, g, w2, b2, layer, eps, r, h, stats, P, L, C):
+    """r, h (and stats, for a backward) of csrc/blocknorm.h; a gate of one row per sample
+    has L rows a sample, of one row per token L = 1."""
+    if P == 0:
+        return
+    with _on(x, f, w1, b1, s, g, w2, b2):
+        call("accunet_blocknorm_fwd", _p(x), _p(f), _p(w1), _p(b1), _p(s), _p(g),
+             _gate_mode(g, L), _p(w2), _p(b2), 1 if layer else 0, eps, _p(r), _p(h), _p(stats),
+             P, L, C, _dt(x), _stream())
+
+
+def blocknorm_bwd(x, f, w1, b1, s, g, w2, layer, stats, dr, dh, dx, df, dg, dpar, P, L, C):
+    if P == 0:
+        dpar.zero_()
+        if dg is not None:
+            dg.zero_()
+        return
+    with _on(x, f, w1, b1, s, g, w2, dr, dh):
+        mode = _gate_mode(g, L)
+        n = int(_lib.load().accunet_blocknorm_ws_elems(P, L, C, mode))
+        ws = workspace(n, x.device)
+        call("accunet_blocknorm_bwd", _p(x), _p(f), _p(w1), _p(b1), _p(s), _p(g), mode, _p(w2),
+             1 if layer else 0, _p(stats), _p(dr), _p(dh), _p(dx), _p(df), _p(dg), _p(dpar),
+             _p(ws), n, P, L, C, _dt(x), _stream())
+
+
+def _gate_mode(g, L) -> int:
+    return 0 if g is None else (2 if L == 1 else 1)
+
+
+class _on:
+    """The device of the given tensors made the current one (they must share it), so the
+    launch and its stream are that device's whatever the caller's current device is."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, first, *rest):
+        dev = first.device
+        for t in rest:
+            if t is not None and t.device != dev:
+                raise _lib.AccError(f"tensors on {dev} and {t.device}")
+        self.guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)

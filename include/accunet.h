@@ -487,6 +487,31 @@ int accunet_relu(const float* x, const float* dy, float* y, long n, void* stream
 int accunet_subsample2(const float* src, float* dst, int B, int H, int W, int C, int bwd,
                        void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Norms around a residual block, fused with its gate and residual scale (token blocks of
+ * the tokenised-MLP models; no reference counterpart). Rows are tokens, x [P][C] of
+ * storage dt, sample b owns rows [b*L, (b+1)*L); 1 <= C <= 8192.
+ *   u = norm(f)*w1 + b1;  r = x + s*g*u;  h = norm(r)*w2 + b2
+ * norm: layer != 0 subtracts the mean, else root-mean-square; eps inside the root. w1, b1,
+ * s, w2, b2 are fp32 [C] or NULL (1, 0, 1, 1, 0). gmode: 0 no gate (g NULL), 1 one row of g
+ * per sample ([P/L][C]), 2 one per token ([P][C]); g has storage dt. f NULL: only
+ * h = norm(x)*w2 + b2 (r NULL). h NULL: no second norm. stats ([P][4] fp32, or NULL when
+ * no backward follows) keeps both norms' mean and 1/sqrt.
+ * Backward: dr / dh (one may be NULL) -> dx, df, dg (g's shape, NULL without a gate) and
+ * dpar [5][C] = dw1, db1, ds, dw2, db2 (the first three only with f). ws: fp32 scratch of
+ * accunet_blocknorm_ws_elems elements.
+ * ------------------------------------------------------------------------- */
+int accunet_blocknorm_fwd(const void* x, const void* f, const float* w1, const float* b1,
+                          const float* s, const void* g, int gmode, const float* w2,
+                          const float* b2, int layer, float eps, void* r, void* h, float* stats,
+                          long P, long L, int C, int dt, void* stream);
+size_t accunet_blocknorm_ws_elems(long P, long L, int C, int gmode);
+int accunet_blocknorm_bwd(const void* x, const void* f, const float* w1, const float* b1,
+                          const float* s, const void* g, int gmode, const float* w2, int layer,
+                          const float* stats, const void* dr, const void* dh, void* dx, void* df,
+                          void* dg, float* dpar, float* ws, size_t ws_elems, long P, long L, int C,
+                          int dt, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
