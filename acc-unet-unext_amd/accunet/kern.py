@@ -640,3 +640,37 @@ class _on:
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+# --------------------------------------- distillation from a teacher's top logits
+def distill_teacher(idx, top, rest, id_, p, tea, count, B, S, V, K, T):
+    with _on(idx, top, rest):
+        call("accunet_distill_teacher", _p(idx), 1 if idx.dtype == torch.int64 else 0, _p(top),
+             _dt(top), _p(rest), _p(id_), _p(p), _p(tea), _p(count), B, S, V, K, T, _stream())
+
+
+def distill_fwd(z, rest, id_, p, tea, state, rowloss, part, B, S, V, K, T, weight, planes):
+    with _on(z, rest, id_):
+        if planes:
+            call("accunet_distill_planes_fwd", _p(z), _p(rest), _p(id_), _p(p), _p(tea),
+                 _p(state), _p(rowloss), _p(part), B, S, V, K, T, weight, _dt(z), _stream())
+            return
+        n = int(_lib.load().accunet_distill_rows_ws_elems(B, V, _dt(z)))
+        ws = workspace(n, z.device)
+        call("accunet_distill_rows_fwd", _p(z), _p(rest), _p(id_), _p(p), _p(tea), _p(state),
+             _p(rowloss), _p(part), _p(ws), n, B, V, K, T, weight, _dt(z), _stream())
+
+
+def distill_bwd(z, id_, p, state, up, up_rows, count, dz, B, S, V, K, T, weight, planes):
+    with _on(z, id_, up):
+        if planes:
+            call("accunet_distill_planes_bwd", _p(z), _p(id_), _p(p), _p(state), _p(up),
+                 1 if up_rows else 0, _p(count), _p(dz), B, S, V, K, T, weight, _dt(z), _stream())
+        else:
+            call("accunet_distill_rows_bwd", _p(z), _p(id_), _p(p), _p(state), _p(up),
+                 1 if up_rows else 0, _p(count), _p(dz), B, V, K, T, weight, _dt(z), _stream())
+
+
+def distill_loss(part, n, count, out):
+    with _on(part):
+        call("accunet_distill_loss", _p(part), n, _p(count), _p(out), _stream())

@@ -12,6 +12,7 @@ import torch
 from torch import nn
 
 from . import ops
+from .distill import topk_distill
 
 
 class WeightedDiceBCE(nn.Module):
@@ -37,3 +38,18 @@ class WeightedDiceBCE(nn.Module):
         targets[targets <= 0] = 0
         dice = ops.weighted_dice_terms(hard, targets)
         return 1.0 - dice
+
+
+class TopKDistill(nn.Module):
+    """Distillation from a teacher's stored top logits (accunet.distill.topk_distill), beside
+    the hard-label loss: forward(logits, top_idx, top_logits, rest=None). dim=1 takes a
+    model's [B, n_classes, H, W] output as it is."""
+
+    def __init__(self, temperature=1.0, weight=1.0, reduction="mean", dim=1):
+        super().__init__()
+        self.temperature, self.weight = temperature, weight
+        self.reduction, self.dim = reduction, dim
+
+    def forward(self, logits, top_idx, top_logits, rest=None):
+        return topk_distill(logits, top_idx, top_logits, rest, self.temperature, self.weight,
+                            self.reduction, self.dim)

@@ -1,0 +1,101 @@
+// Distillation from a teacher's top logits (distill.hip, distill_rows.hip).
+//
+// Row i: student logits z[0..V), the teacher's entries (idx_k, t_k), k < K, an optional
+// mass `rest` of the teacher outside them, temperature T.
+//   p_k   = (1 - rest) * softmax(t / T)_k over the entries with 0 <= idx_k < V
+//   q     = softmax(z / T) over all V classes, q_rest = sum of q over classes not listed
+//   loss  = T^2 * [ sum_k p_k (log p_k - log q_idx_k) + rest (log rest - log q_rest) ]
+//   dloss/dz_j = T * (q_j - p_j)                  listed (p_j: the sum over its entries)
+//              = T * (q_j - rest * q_j / q_rest)  not listed
+// A row without a valid entry (or whose valid t are all -inf) has loss 0 and gradient 0
+// and is not counted by the mean.
+//
+// Arithmetic is in base 2: with c = log2(e) / T a softmax term is 2^(z*c - m*c), one fma
+// and one v_exp_f32; m*c is rounded once and enters numerator and sum alike, so it cancels.
+// q_rest is summed over the classes not listed, never as 1 - sum of the others, and a row's
+// state keeps it relative to the largest such class, so it may be far below fp32's range:
+//   not listed: dz = 2^(z*c - mu) * cu,  cu = 2^(mu - m) / S - rest / S_rest
+//   listed:     dz = 2^(z*c - m) / S - p
+#pragma once
+#include "common.h"
+
+#define DT_MAX_K 256
+#define DT_MAX_V (1 << 30)
+#define DT_LN2 0.69314718055994531f
+#define DT_LOG2E 1.4426950408889634
+
+// one row's state between the passes
+//   x: mu, y: cu, z: m (all * c, base 2), w: 1/S, or DT_EMPTY for a row that does not count
+#define DT_EMPTY (-1.f)
+
+ACC_DEV float dt_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
+// 2^((m - M) * c), 1 where both are the same infinity
+ACC_DEV float dt_rescale(float m, float M, float c) { return m == M ? 1.f : dt_exp2((m - M) * c); }
+// m * c as a reference for exponents; 0 where no class is left (every term is 2^-inf then)
+ACC_DEV float dt_ref(float m, float c) { return m == -INFINITY ? 0.f : m * c; }
+// (m, s) joined with (m2, s2)
+ACC_DEV void dt_join(float& m, float& s, float m2, float s2, float c) {
+  const float M = fmaxf(m, m2);
+  s = s * dt_rescale(m, M, c) + s2 * dt_rescale(m2, M, c);
+  m = M;
+}
+// LDS written by one lane of a wave and read by another of the same wave
+ACC_DEV void dt_wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+ACC_DEV float dt_wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+ACC_DEV float dt_wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+ACC_DEV void dt_wave_join(float& m, float& s, float c) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+    dt_join(m, s, m2, s2, c);
+  }
+}
+
+// The row's state and loss (base 2, before T^2 ln 2) once (m, s) over the streamed classes,
+// and over the listed ones if they were left out (REST), are known. `dot` is the caller's
+// sum over listed entries of p * log2 q.
+struct DtRow {
+  float4 state;
+  float M, log2S;
+};
+ACC_DEV DtRow dt_row_state(float m, float s, float mr, float sr, float rest, bool has_rest, float c) {
+  DtRow o;
+  const float ref = dt_ref(m, c);
+  o.M = ref;
+  o.log2S = log2f(s);
+  o.state.z = ref;
+  o.state.w = 1.f / s;
+  o.state.x = ref;
+  o.state.y = o.state.w;
+  if (has_rest) {
+    o.state.x = dt_ref(mr, c);
+    o.state.y = sr > 0.f ? dt_rescale(mr, m, c) / s - rest / sr : (sr == 0.f ? 0.f : sr);
+  }
+  return o;
+}
+
+// the step from a row's sums to its gradient: weight * T * upstream / rows counted
+struct DtScale {
+  const float* up;      // upstream gradient: one value, or one per row (up_rows)
+  int up_rows;
+  const int* count;     // rows counted (mean), or null
+  float k;              // weight * T
+};
+ACC_DEV float dt_scale(const DtScale& g, long row) {
+  float v = g.k;
+  if (g.up) v *= g.up[g.up_rows ? row : 0];
+  if (g.count) v /= (float)max(*g.count, 1);
+  return v;
+}

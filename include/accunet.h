@@ -512,6 +512,46 @@ int accunet_blocknorm_bwd(const void* x, const void* f, const float* w1, const f
                           void* dg, float* dpar, float* ws, size_t ws_elems, long P, long L, int C,
                           int dt, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Distillation loss from a teacher's top logits, forward and backward (beside the
+ * segmentation loss; no reference counterpart). Logits z of storage dt with V classes:
+ * "rows" z [R][V], or "planes" z [B][V][S] (classes on the channel axis; V <= 1024). The
+ * teacher's K <= 256 entries a row: idx (int32, or int64 with idx64), top (storage top_dt),
+ * [R][K] or [B][K][S]; an index outside [0, V) is padding. rest (fp32, one a row, or NULL):
+ * the teacher's mass outside its entries. T > 0 the temperature, weight a factor of the loss.
+ *   p = (1 - rest) softmax(top / T), q = softmax(z / T)
+ *   loss = weight T^2 [sum p (log p - log q) + rest (log rest - log q(not listed))]
+ * A row without a valid entry has loss 0 and gradient 0.
+ *   accunet_distill_teacher: id [.][K] int32 (each class once, -1 elsewhere), p [.][K] fp32,
+ *     tea [rows][2] fp32, *count (int32, zeroed by the caller) += rows with an entry. S = 1
+ *     for "rows" (B = R).
+ *   accunet_distill_rows_fwd / _planes_fwd: state [rows][4] fp32, rowloss [rows] fp32 (or
+ *     NULL), part fp64 (rows: [R], planes: [ceil(B*S/256)]); ws: fp32 scratch of
+ *     accunet_distill_rows_ws_elems elements.
+ *   accunet_distill_loss: out = sum of the n values of part, / *count where count is given.
+ *   accunet_distill_rows_bwd / _planes_bwd: dz (z's type, shape and address modulo 16),
+ *     scaled by the upstream gradient up (one value, or one a row with up_rows; NULL: 1) and
+ *     1 / *count where count is given.
+ * ------------------------------------------------------------------------- */
+int accunet_distill_teacher(const void* idx, int idx64, const void* top, int top_dt,
+                            const float* rest, int* id, float* p, float* tea, int* count, long B,
+                            long S, int V, int K, float T, void* stream);
+size_t accunet_distill_rows_ws_elems(long R, int V, int dt);
+int accunet_distill_rows_fwd(const void* z, const float* rest, const int* id, const float* p,
+                             const float* tea, float* state, float* rowloss, double* part,
+                             float* ws, size_t ws_elems, long R, int V, int K, float T,
+                             float weight, int dt, void* stream);
+int accunet_distill_rows_bwd(const void* z, const int* id, const float* p, const float* state,
+                             const float* up, int up_rows, const int* count, void* dz, long R,
+                             int V, int K, float T, float weight, int dt, void* stream);
+int accunet_distill_planes_fwd(const void* z, const float* rest, const int* id, const float* p,
+                               const float* tea, float* state, float* rowloss, double* part, long B,
+                               long S, int V, int K, float T, float weight, int dt, void* stream);
+int accunet_distill_planes_bwd(const void* z, const int* id, const float* p, const float* state,
+                               const float* up, int up_rows, const int* count, void* dz, long B,
+                               long S, int V, int K, float T, float weight, int dt, void* stream);
+int accunet_distill_loss(const double* part, long n, const int* count, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
