@@ -23,20 +23,31 @@ from ._lib import AccError
 KINDS = ("layer", "rms")
 
 
+def _forward(x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L, keep):
+    C = x.shape[-1]
+    P = x.numel() // C
+    r = torch.empty_like(x) if f is not None else None
+    h = torch.empty_like(x) if want_h else None
+    stats = torch.empty(P, 4, dtype=torch.float32, device=x.device) if keep else None
+    kern.blocknorm_fwd(x, f, w1, b1, s, g, w2, b2, layer, eps, r, h, stats, P, L, C)
+    return r, h, stats
+
+
+def _apply(*args):
+    """The formulas on checked arguments; the autograd node only where a gradient may flow."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
+        return _BlockNormFn.apply(*args)
+    return _forward(*args, False)[:2]
+
+
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L):
+        r, h, stats = _forward(x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L, True)
         C = x.shape[-1]
-        P = x.numel() // C
-        keep = any(ctx.needs_input_grad)
-        r = torch.empty_like(x) if f is not None else None
-        h = torch.empty_like(x) if want_h else None
-        stats = torch.empty(P, 4, dtype=torch.float32, device=x.device) if keep else None
-        kern.blocknorm_fwd(x, f, w1, b1, s, g, w2, b2, layer, eps, r, h, stats, P, L, C)
-        if keep:
-            ctx.save_for_backward(x, f, w1, b1, s, g, w2, stats)
-            ctx.cfg = (layer, P, L, C)
-            ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, f, w1, b1, s, g, w2, stats)
+        ctx.cfg = (layer, x.numel() // C, L, C)
+        ctx.set_materialize_grads(False)
         return r, h
 
     @staticmethod
@@ -114,8 +125,8 @@ def sandwich_norm(x, f, post_weight=None, post_bias=None, scale=None, gate=None,
             ((post_weight, "post_weight"), (post_bias, "post_bias"), (scale, "scale"),
              (pre_weight, "pre_weight"), (pre_bias, "pre_bias"))]
     f = _act(f, "sandwich_norm f", x)
-    return _BlockNormFn.apply(x.contiguous(), f, args[0], args[1], args[2], gate, args[3],
-                              args[4], kind == "layer", float(eps), bool(pre), L)
+    return _apply(x.contiguous(), f, args[0], args[1], args[2], gate, args[3], args[4],
+                  kind == "layer", float(eps), bool(pre), L)
 
 
 def norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
@@ -123,8 +134,8 @@ def norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
     _check_x(x, kind)
     C = x.shape[-1]
     w, b = _param(weight, C, "weight", x), _param(bias, C, "bias", x)
-    return _BlockNormFn.apply(x.contiguous(), None, None, None, None, None, w, b,
-                              kind == "layer", float(eps), True, x.numel() // C)[1]
+    return _apply(x.contiguous(), None, None, None, None, None, w, b, kind == "layer",
+                  float(eps), True, x.numel() // C)[1]
 
 
 class SandwichNorm(nn.Module):

@@ -1,0 +1,188 @@
+"""Linear layer in 8-bit floating point with a scale for each block of 128.
+
+Values are e4m3; a block's scale is 2^e, e the least integer with amax <= 448 * 2^e, so
+scaling is exact and a value is rounded once, to nearest even. Activations and output
+gradients are quantised in blocks of 1 x 128 along the contracted axis, weights in blocks of
+128 x 128. With Q(.) the quantised values and fp32 sums:
+
+    y  = Q(x) Q(w)^T + bias        contracted over the input features
+    dx = Q(dy) Q(w)                over the output features
+    dw = Q(dy)^T Q(x)              over the tokens, both quantised along the tokens
+    db = sum of dy over the tokens
+
+Activations are float32 or bfloat16; weights, biases and their gradients are float32. An
+element that is not finite becomes NaN; scales stop at 2^-126 and 2^120. Non-contiguous
+inputs are copied (csrc/fp8.h, csrc/fp8_quant.hip, csrc/fp8_gemm.hip).
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import kern
+from ._lib import AccError
+
+BLOCK = 128
+
+
+def _pad(n):
+    return -(-n // BLOCK) * BLOCK
+
+
+def _pitch(n):
+    return -(-_pad(n) // (4 * BLOCK)) * 4
+
+
+class Fp8Blocks:
+    """A quantised matrix [rows, cols], contracted along its columns: `q` float8_e4m3fn
+    [rows, cols rounded up to 128], `s` uint8 [rows, blocks rounded up to 4] (biased
+    exponents). `t` is the transposed matrix where it was asked for."""
+
+    __slots__ = ("q", "s", "rows", "cols", "square", "t")
+
+    def __init__(self, q, s, rows, cols, square, t=None):
+        self.q, self.s, self.rows, self.cols, self.square, self.t = q, s, rows, cols, square, t
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def values(self):
+        """The float32 values that the matrix stands for."""
+        scale = torch.ldexp(torch.ones((), device=self.device), self.s.int() - 127)
+        scale = scale.repeat_interleave(BLOCK, 1)[:, :self.cols]
+        return self.q[:, :self.cols].float() * scale
+
+
+def _new(rows, cols, dev):
+    return (torch.empty(rows, _pad(cols), dtype=torch.float8_e4m3fn, device=dev),
+            torch.empty(rows, _pitch(cols), dtype=torch.uint8, device=dev))
+
+
+def _quantize(x, R, C, square=False, rows=True, cols=False, colsum=None):
+    """(q, s), (qt, st) of x [R, C]; the column sums into `colsum`."""
+    q, s = _new(R, C, x.device) if rows else (None, None)
+    qt, st = _new(C, R, x.device) if cols else (None, None)
+    kern.fp8_quantize(x, square, q, s, qt, st, colsum, R, C)
+    return (q, s), (qt, st)
+
+
+def quantize(x, square=False, transposed=False):
+    """Fp8Blocks of x [R, C] (float32 or bfloat16): blocks of 1 x 128, with square=True of
+    128 x 128 (weights). transposed=True keeps the transposed matrix too, which the
+    gradient of a frozen weight's input needs."""
+    kern._check(x, "fp8.quantize x", act=True)
+    if x.dim() != 2 or x.numel() == 0:
+        raise AccError(f"fp8.quantize: a matrix with elements expected, got {tuple(x.shape)}")
+    if transposed and not square:
+        raise ValueError("fp8.quantize: transposed needs square blocks")
+    R, C = x.shape
+    (q, s), (qt, st) = _quantize(x.detach().contiguous(), R, C, square, cols=transposed)
+    t = Fp8Blocks(qt, st, C, R, True) if transposed else None
+    return Fp8Blocks(q, s, R, C, square, t)
+
+
+def _gemm(a, b, M, N, K, bias, dtype):
+    c = torch.empty(M, N, dtype=dtype, device=a[0].device)
+    kern.fp8_gemm(a[0], a[1], b[0], b[1], bias, c, M, N, K)
+    return c
+
+
+def _forward(x, weight, bias, wq, N, need_x=False, need_w=False, wt=None):
+    """y, and what the gradients need: the transposed x and weight."""
+    K = x.shape[-1]
+    M = x.numel() // K
+    xt = (None, None)
+    if M:
+        xq, xt = _quantize(x, M, K, cols=need_w)
+    if weight is not None and (M or need_x):
+        wq, wt = _quantize(weight, N, K, square=True, cols=need_x)
+    y = _gemm(xq, wq, M, N, K, bias, x.dtype) if M else x.new_empty(0, N)
+    return y.view(*x.shape[:-1], N), xt, (wt if need_x else (None, None))
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, wq, wt, N):
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        y, xt, wt = _forward(x, weight, bias, wq, N, need_x, need_w, wt)
+        ctx.save_for_backward(*xt, *wt)
+        K = x.shape[-1]
+        ctx.cfg = (x.numel() // K, N, K, x.shape, x.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        qt, st, wqt, wst = ctx.saved_tensors
+        M, N, K, shape, dtype = ctx.cfg
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = dy.device
+        dx = dw = db = None
+        if M == 0:
+            return (torch.empty(shape, dtype=dtype, device=dev) if need_x else None,
+                    torch.zeros(N, K, device=dev) if need_w else None,
+                    torch.zeros(N, device=dev) if need_b else None, None, None, None)
+        dy = dy.contiguous()
+        db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
+        # the bias alone needs no quantised matrix, but shares the pass that makes one
+        rows, cols = _quantize(dy, M, N, rows=need_x or not need_w, cols=need_w, colsum=db)
+        if need_x:
+            dx = _gemm(rows, (wqt, wst), M, K, N, None, dtype).view(shape)
+        if need_w:
+            dw = _gemm(cols, (qt, st), N, K, M, None, torch.float32)
+        return dx, dw, db, None, None, None
+
+
+def linear(x, weight, bias=None):
+    """The layer of the module docstring on x [..., K]: weight float32 [N, K], or a frozen
+    one as quantize(w, square=True) left it; bias float32 [N] or None. Returns x's type."""
+    kern._check(x, "fp8.linear x", act=True)
+    frozen = isinstance(weight, Fp8Blocks)
+    if not frozen:
+        kern._check(weight, "fp8.linear weight")
+        if weight.dim() != 2:
+            raise AccError(f"fp8.linear: weight [N, K] expected, got {tuple(weight.shape)}")
+    N, K = weight.shape
+    if x.dim() < 1 or x.shape[-1] != K or N < 1 or K < 1:
+        raise AccError(f"fp8.linear: x {tuple(x.shape)} and weight {(N, K)} do not match")
+    if weight.device != x.device:
+        raise AccError(f"fp8.linear: weight on {weight.device}, x on {x.device}")
+    if bias is not None:
+        kern._check(bias, "fp8.linear bias")
+        if tuple(bias.shape) != (N,) or bias.device != x.device:
+            raise AccError(f"fp8.linear: bias {tuple(bias.shape)} on {bias.device}, expected "
+                           f"{(N,)} on {x.device}")
+        bias = bias.contiguous()
+    grad = torch.is_grad_enabled() and (
+        x.requires_grad or (not frozen and weight.requires_grad)
+        or (bias is not None and bias.requires_grad))
+    x = x.contiguous()
+    wq = wt = None
+    if frozen:
+        if not weight.square:
+            raise AccError("fp8.linear: a frozen weight needs blocks of 128 x 128 "
+                           "(quantize(w, square=True))")
+        wq = (weight.q, weight.s)
+        if weight.t is not None:
+            wt = (weight.t.q, weight.t.s)
+        elif grad and x.requires_grad:
+            raise AccError("fp8.linear: the gradient of x needs the transposed weight "
+                           "(quantize(w, square=True, transposed=True))")
+        weight = None
+    else:
+        weight = weight.contiguous()
+    if not grad:
+        return _forward(x, weight, bias, wq, N)[0]
+    return _LinearFn.apply(x, weight, bias, wq, wt, N)
+
+
+class Linear(nn.Linear):
+    """nn.Linear (same parameters and state_dict) whose products run in 8 bits."""
+
+    def forward(self, x):
+        return linear(x, self.weight, self.bias)

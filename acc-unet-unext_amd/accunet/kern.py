@@ -674,3 +674,20 @@ def distill_bwd(z, id_, p, state, up, up_rows, count, dz, B, S, V, K, T, weight,
 def distill_loss(part, n, count, out):
     with _on(part):
         call("accunet_distill_loss", _p(part), n, _p(count), _p(out), _stream())
+
+
+# ------------------------------------------------------------- 8-bit linear layer
+def fp8_quantize(x, square, q, s, qt, st, sum_, R, C):
+    with _on(x):
+        n = int(_lib.load().accunet_fp8_sum_ws_elems(R, C)) if sum_ is not None else 0
+        ws = workspace(n, x.device) if n else None
+        call("accunet_fp8_quantize", _p(x), 1 if square else 0, _p(q), _p(s), _p(qt), _p(st),
+             _p(sum_), _p(ws), n, R, C, _dt(x), _stream())
+
+
+def fp8_gemm(a, sa, b, sb, bias, c, M, N, K):
+    with _on(a, sa, b, sb, bias, c):
+        n = int(_lib.load().accunet_fp8_gemm_ws_elems(M, N, K))
+        ws = workspace(n, a.device) if n else None
+        call("accunet_fp8_gemm", _p(a), _p(sa), _p(b), _p(sb), _p(bias), _p(c), _p(ws), n, M, N, K,
+             _dt(c), _stream())

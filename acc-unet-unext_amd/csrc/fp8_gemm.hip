@@ -1,0 +1,269 @@
+// The 8-bit linear layer's product: C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]) over two
+// quantised matrices contracted along their rows (formats in fp8.h), fp32 accumulators.
+//
+// Two forms of the inner product:
+//   bf16 outputs: v_mfma_scale_f32_16x16x128_f8f6f4 contracts one 128-block of 16 rows of
+//     each side, the block scales (one exponent byte a row) applied by the instruction, so a
+//     k-tile is one scale block. Measured on the card: the instruction aligns groups of 8
+//     products and keeps 13 bits below the largest of a group (groups and accumulator join in
+//     fp32). The loss, about 2e-5 of a random sum's size, is a hundredth of bf16's rounding.
+//   fp32 outputs (WIDE): the bytes become bf16 in registers, scale included, which is exact,
+//     and v_mfma_f32_16x16x32_bf16 sums in fp32 (its products were exact to 2^-23 in the same
+//     measurement). Half the matrix rate; a value times its scale must stay a normal fp32.
+// The first operand is B: a lane then holds 4 neighbouring n of one m and
+// stores them at once. Tiles go global -> LDS by 16-byte DMA without registers; a tile row's
+// eight 16-byte chunks are permuted by (row >> 1) & 7 through the source address, so 16 rows
+// of one chunk, which a fragment read takes at once, cover all 64 banks. The scale dwords of
+// four k-tiles ride along every fourth tile. Rows past the end read the last row; what they
+// yield is not stored.
+#include "fp8.h"
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+// 8 e4m3 bytes as bf16, times a power of two
+ACC_DEV v8b fp8_widen(int lo, int hi, float scale) {
+  const v2b a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, false);
+  const v2b b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, true);
+  const v2b c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, false);
+  const v2b d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, true);
+  return (v8b){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Lane i copies 16 (4) bytes from its `src` to lds + 16 i (4 i), lds the same for the wave.
+// From inline asm: the compiler would otherwise wait for every copy before any LDS read of
+// the array. The wave waits for its copies itself, before the barrier that publishes them.
+ACC_DEV unsigned fp8_lds_addr(const void* p) {
+  return __builtin_amdgcn_readfirstlane(
+      (unsigned)(size_t)(__attribute__((address_space(3))) const void*)p);
+}
+ACC_DEV void fp8_dma16(const void* src, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
+               "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
+}
+ACC_DEV void fp8_dma4(const void* src, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
+               "global_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
+}
+
+struct Fp8GemmArgs {
+  const unsigned char *a, *sa, *b, *sb;
+  void* c;
+  const float* bias;
+  float* slab;  // split: [splits][M][N] partial sums
+  long M, N;
+  int KP, SP, kt_per;  // k-tiles per split (a multiple of 4)
+  int tiles_n, vec;
+};
+
+template <typename T>
+ACC_DEV void fp8_store4(T* p, const float (&v)[4], int n, bool vec) {
+  if (vec && n >= 4) {
+    stq(p, make_float4(v[0], v[1], v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) st1(p + i, v[i]);
+  }
+}
+
+template <typename T, bool SPLIT, bool WIDE>
+__global__ void __launch_bounds__(256, 2)
+fp8_gemm_kernel(const Fp8GemmArgs g) {
+  constexpr int BM = 128, BN = 128;
+  __shared__ __attribute__((aligned(1024))) unsigned char sA[2][BM * 128];
+  __shared__ __attribute__((aligned(1024))) unsigned char sB[2][BN * 128];
+  __shared__ __attribute__((aligned(1024))) unsigned sS[2][BM + BN];
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+  const long m0 = (long)(blockIdx.x / g.tiles_n) * BM;
+  const long n0 = (long)(blockIdx.x % g.tiles_n) * BN;
+  const int kt0 = SPLIT ? blockIdx.z * g.kt_per : 0;
+  const int kt1 = SPLIT ? min(g.KP / 128, kt0 + g.kt_per) : g.KP / 128;
+
+  const unsigned char *pa[4], *pb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = wave * 32 + i * 8 + (lane >> 3);
+    const int ch = (lane & 7) ^ ((r >> 1) & 7);
+    pa[i] = g.a + min(m0 + r, g.M - 1) * g.KP + ch * 16 + (long)kt0 * 128;
+    pb[i] = g.b + min(n0 + r, g.N - 1) * g.KP + ch * 16 + (long)kt0 * 128;
+  }
+  const unsigned char* ps = wave < 2 ? g.sa + min(m0 + t, g.M - 1) * g.SP
+                                     : g.sb + min(n0 + t - BM, g.N - 1) * g.SP;
+  auto stage = [&](int kt) {
+    const int buf = (kt - kt0) & 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      fp8_dma16(pa[i], fp8_lds_addr(&sA[buf][(wave * 32 + i * 8) * 128]));
+      fp8_dma16(pb[i], fp8_lds_addr(&sB[buf][(wave * 32 + i * 8) * 128]));
+      pa[i] += 128;
+      pb[i] += 128;
+    }
+    if (((kt - kt0) & 3) == 0) fp8_dma4(ps + kt, fp8_lds_addr(&sS[((kt - kt0) >> 2) & 1][wave * 64]));
+  };
+
+  v4f acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  unsigned sa[4], sb[4];
+  const int l15 = lane & 15, kg = lane >> 4;
+  auto frag = [&](const unsigned char* tile, int r) {
+    const int sw = (r >> 1) & 7;
+    const v4i lo = *reinterpret_cast<const v4i*>(tile + r * 128 + ((2 * kg) ^ sw) * 16);
+    const v4i hi = *reinterpret_cast<const v4i*>(tile + r * 128 + ((2 * kg + 1) ^ sw) * 16);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  if (kt0 < kt1) stage(kt0);
+  for (int kt = kt0; kt < kt1; ++kt) {
+    // this wave's copies have landed and its reads of the other buffer are done; behind
+    // the barrier both hold for every wave
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + 1 < kt1) stage(kt + 1);
+    const int buf = (kt - kt0) & 1, q = (kt - kt0) & 3;
+    if (q == 0) {
+      const unsigned* sc = sS[((kt - kt0) >> 2) & 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sa[i] = sc[wm * 64 + i * 16 + l15];
+        sb[i] = sc[BM + wn * 64 + i * 16 + l15];
+      }
+    }
+    v8i fa[4], fb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      fa[i] = frag(sA[buf], wm * 64 + i * 16 + l15);
+      fb[i] = frag(sB[buf], wn * 64 + i * 16 + l15);
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v8b wb[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          wb[j] = fp8_widen(fb[j][2 * k], fb[j][2 * k + 1], __uint_as_float((sb[j] & 255u) << 23));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v8b wa =
+              fp8_widen(fa[i][2 * k], fa[i][2 * k + 1], __uint_as_float((sa[i] & 255u) << 23));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], wa, acc[i][j], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              fb[j], fa[i], acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sa[i] >>= 8;
+      sb[i] >>= 8;
+    }
+  }
+
+  // lane: m = l15 of the fragment, n = 4 kg .. + 3
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long m = m0 + wm * 64 + i * 16 + l15;
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long n = n0 + wn * 64 + j * 16 + kg * 4;
+      const int left = (int)min(4L, g.N - n);
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+      if (SPLIT) {
+        fp8_store4(g.slab + ((long)blockIdx.z * g.M + m) * g.N + n, v, left, g.vec);
+      } else {
+        if (g.bias)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < left) v[e] += g.bias[n + e];
+        fp8_store4((T*)g.c + m * g.N + n, v, left, g.vec);
+      }
+    }
+  }
+}
+
+// C = sum of the slabs in order (+ bias)
+template <typename T>
+__global__ void __launch_bounds__(256)
+fp8_join_kernel(const float* __restrict__ slab, int splits, const float* __restrict__ bias,
+                T* __restrict__ c, long n, long N) {
+  const long e = blockIdx.x * 256L + threadIdx.x;
+  if (e >= n) return;
+  float v[1] = {0.f};
+  ordered_strided_sum<4>(v, 0, splits, 1, [&](int k, float (&o)[1]) { o[0] = slab[k * n + e]; });
+  if (bias) v[0] += bias[e % N];
+  st1(c + e, v[0]);
+}
+
+// Splits of the contraction: where the output has fewer than 256 tiles (one a CU), enough
+// for two a CU, each of four k-tiles (one dword of scales) at least.
+static int fp8_splits(long M, long N, long K) {
+  const long tiles = ((M + 127) / 128) * ((N + 127) / 128);
+  const long quads = (fp8_pad(K) / 128 + 3) / 4;
+  if (tiles >= 256 || quads < 2) return 1;
+  long s = min((512 + tiles - 1) / tiles, quads);
+  const long per = (quads + s - 1) / s;
+  return (int)((quads + per - 1) / per);
+}
+
+extern "C" size_t accunet_fp8_gemm_ws_elems(long M, long N, long K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const int s = fp8_splits(M, N, K);
+  return s > 1 ? (size_t)s * M * N : 0;
+}
+
+extern "C" int accunet_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb,
+                                const float* bias, void* c, float* ws, size_t ws_elems, long M,
+                                long N, long K, int cdt, void* stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > (1L << 30)) return ACC_EBADSHAPE;
+  const long tm = (M + 127) / 128, tn = (N + 127) / 128;
+  if (tn > 0x7fffffffL || tm * tn > 0x7fffffffL) return ACC_EBADSHAPE;
+  if (!a || !sa || !b || !sb || !c) return ACC_EBADARG;
+  if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)sa | (uintptr_t)sb) & 3) return ACC_EBADARG;
+  if (ws_elems < accunet_fp8_gemm_ws_elems(M, N, K)) return ACC_EBADARG;
+  Fp8GemmArgs g;
+  g.a = (const unsigned char*)a; g.sa = (const unsigned char*)sa;
+  g.b = (const unsigned char*)b; g.sb = (const unsigned char*)sb;
+  g.c = c; g.bias = bias; g.slab = ws;
+  g.M = M; g.N = N; g.KP = (int)fp8_pad(K); g.SP = (int)fp8_scale_pitch(K);
+  g.tiles_n = (int)tn;
+  const int splits = fp8_splits(M, N, K);
+  const int quads = (g.KP / 128 + 3) / 4;
+  g.kt_per = (quads + splits - 1) / splits * 4;
+  hipStream_t st = (hipStream_t)stream;
+  const int rc = with_dt(cdt, [&](auto tag) {
+    using T = decltype(tag);
+    const dim3 grid((unsigned)(tm * tn), 1, splits);
+    if (splits > 1) {
+      g.vec = N % 4 == 0 && ((uintptr_t)ws & 15) == 0;
+      hipLaunchKernelGGL((fp8_gemm_kernel<T, true, sizeof(T) == 4>), grid, dim3(256), 0, st, g);
+      hipLaunchKernelGGL(fp8_join_kernel<T>, dim3((unsigned)((M * N + 255) / 256)), dim3(256), 0,
+                         st, ws, splits, bias, (T*)c, M * N, N);
+    } else {
+      g.vec = N % 4 == 0 && ((uintptr_t)c & (4 * sizeof(T) - 1)) == 0;
+      hipLaunchKernelGGL((fp8_gemm_kernel<T, false, sizeof(T) == 4>), grid, dim3(256), 0, st, g);
+    }
+  });
+  if (rc != ACC_OK) return rc;
+  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
+}

@@ -1,0 +1,229 @@
+// Quantisers of the 8-bit linear layer; formats in fp8.h. Bound by memory: the input is
+// read once, whatever is made of it (rows, transposed rows, column sums), one byte an
+// element is written for each form.
+#include "fp8.h"
+
+template <typename T>
+ACC_DEV void fp8_load8(const T* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    const float4 a = ldq(p), b = ldq(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = u < n ? ld1(p + u) : 0.f;
+  }
+}
+
+// Rows only: 16 threads a block of 128, 8 elements each. A thread past the scale pitch's
+// last block leaves; one in the padding writes the padding.
+template <typename T>
+__global__ void __launch_bounds__(256)
+fp8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
+                unsigned char* __restrict__ s, long R, int C, int CP, int SP, int vec) {
+  const int per = SP * 16;  // threads a row
+  const long g = blockIdx.x * 256L + threadIdx.x;
+  const long row = g / per;
+  if (row >= R) return;
+  const int t = (int)(g - row * per);
+  const int c = t * 8;
+  float v[8];
+  fp8_load8(x + row * C + c, C - c, vec, v);
+  unsigned m = 0u;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) m = max(m, fp8_finite_bits(v[u]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+  const int e = fp8_scale_byte(m);
+  const float inv = fp8_inverse(e);
+  if (c < CP) {
+    uint2 w;
+    w.x = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    w.y = fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    *reinterpret_cast<uint2*>(q + row * CP + c) = w;
+  }
+  if ((t & 15) == 0) s[row * SP + (t >> 4)] = (unsigned char)e;
+}
+
+// A 128 x 128 tile: thread t holds columns 8 (t % 16) .. + 7 of rows t / 16 + 16 i.
+//   q, s     blocks 1 x 128 along the rows          (square: the tile is one block)
+//   qt, st   the transposed matrix [C][RP], blocks 1 x 128 along the rows of x
+//   sum      [tiles of rows][C] column sums
+// The transposed bytes go through LDS: [column][row], a column's 128 bytes padded to 132 so
+// that the 16 columns a wave writes at once lie in different banks.
+#define FP8_TP 132
+template <typename T>
+__global__ void __launch_bounds__(256)
+fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
+                unsigned char* __restrict__ s, unsigned char* __restrict__ qt,
+                unsigned char* __restrict__ st, float* __restrict__ sum, long R, int C, int CP,
+                int SP, long RP, int SPT, int square, int vec) {
+  __shared__ __attribute__((aligned(16))) unsigned char tile[128 * FP8_TP];
+  __shared__ unsigned cmax[16][128];
+  __shared__ unsigned wmax[4];
+  __shared__ unsigned char cb[128];
+  float (*csum)[128] = reinterpret_cast<float (*)[128]>(tile);
+  const int t = threadIdx.x, cg = t & 15, rg = t >> 4;
+  const long r0 = (long)blockIdx.x * 128;
+  const int c0 = blockIdx.y * 128, c = c0 + cg * 8;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const long r = r0 + rg + 16 * i;
+    fp8_load8(x + r * C + c, r < R ? C - c : 0, vec, v[i]);
+  }
+  int e[8];
+  unsigned all = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    unsigned m = 0u;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m = max(m, fp8_finite_bits(v[i][u]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+    e[i] = fp8_scale_byte(m);
+    all = max(all, m);
+  }
+  if (square) {
+    all = max(all, (unsigned)__shfl_xor((int)all, 16));
+    all = max(all, (unsigned)__shfl_xor((int)all, 32));
+    if ((t & 63) == 0) wmax[t >> 6] = all;
+    __syncthreads();
+    const int eb = fp8_scale_byte(max(max(wmax[0], wmax[1]), max(wmax[2], wmax[3])));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = eb;
+  }
+  if (q) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long r = r0 + rg + 16 * i;
+      if (r >= R) continue;
+      const float inv = fp8_inverse(e[i]);
+      uint2 w;
+      w.x = fp8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+      w.y = fp8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+      *reinterpret_cast<uint2*>(q + r * CP + c) = w;
+      if (cg == 0) s[r * SP + blockIdx.y] = (unsigned char)e[i];
+      // the scale row's padding, written once
+      if (cg == 0 && (int)blockIdx.y == CP / 128 - 1)
+        for (int b = CP / 128; b < SP; ++b) s[r * SP + b] = (unsigned char)FP8_ONE;
+    }
+  }
+  if (qt) {
+    float inv[8];
+    if (square) {
+      const float iv = fp8_inverse(e[0]);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) inv[u] = iv;
+      if (t < 128) cb[t] = (unsigned char)e[0];
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        unsigned m = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, fp8_finite_bits(v[i][u]));
+        cmax[rg][cg * 8 + u] = m;
+      }
+      __syncthreads();
+      if (t < 128) {
+        unsigned m = 0u;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) m = max(m, cmax[k][t]);
+        cb[t] = (unsigned char)fp8_scale_byte(m);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 8; ++u) inv[u] = fp8_inverse(cb[cg * 8 + u]);
+    }
+    // rows rg + 16 i of this thread: byte (column, row)
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        tile[(cg * 8 + u) * FP8_TP + rg + 16 * i] =
+            (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(v[i][u] * inv[u], 0.f, 0, false);
+    __syncthreads();
+    // 8 threads a column, 16 bytes each
+    for (int k = t; k < 128 * 8; k += 256) {
+      const int cc = k >> 3, b = (k & 7) * 16;
+      if (c0 + cc >= C) continue;
+      const unsigned* src = reinterpret_cast<const unsigned*>(tile + cc * FP8_TP + b);
+      *reinterpret_cast<uint4*>(qt + (long)(c0 + cc) * RP + r0 + b) =
+          make_uint4(src[0], src[1], src[2], src[3]);
+    }
+    if (t < 128 && c0 + t < C) {
+      unsigned char* so = st + (long)(c0 + t) * SPT;
+      so[blockIdx.x] = cb[t];
+      if ((long)blockIdx.x == RP / 128 - 1)
+        for (int b = (int)(RP / 128); b < SPT; ++b) so[b] = (unsigned char)FP8_ONE;
+    }
+  }
+  if (sum) {
+    __syncthreads();  // tile is read above
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a += v[i][u];
+      csum[rg][cg * 8 + u] = a;
+    }
+    __syncthreads();
+    if (t < 128 && c0 + t < C) {
+      float a = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) a += csum[k][t];
+      sum[(long)blockIdx.x * C + c0 + t] = a;
+    }
+  }
+}
+
+// out[c] = sum over n rows of part [n][C] in order
+__global__ void __launch_bounds__(256)
+fp8_colsum_kernel(const float* __restrict__ part, long n, int C, float* __restrict__ out) {
+  __shared__ double red[4][64];
+  const int cl = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + cl;
+  double v[1] = {0.0};
+  if (c < C)
+    ordered_strided_sum<4>(v, g, (int)n, 4, [&](int r, double (&o)[1]) { o[0] = part[(long)r * C + c]; });
+  red[g][cl] = v[0];
+  __syncthreads();
+  if (g == 0 && c < C) out[c] = (float)(((red[0][cl] + red[1][cl]) + red[2][cl]) + red[3][cl]);
+}
+
+extern "C" size_t accunet_fp8_sum_ws_elems(long R, int C) {
+  return R > 0 && C > 0 ? (size_t)((R + 127) / 128) * C : 0;
+}
+
+extern "C" int accunet_fp8_quantize(const void* x, int square, void* q, void* s, void* qt, void* st,
+                                    float* sum, float* ws, size_t ws_elems, long R, int C, int dt,
+                                    void* stream) {
+  if (R <= 0 || C <= 0 || (R + 127) / 128 > 0x7fffffffL || C > 65535 * 128) return ACC_EBADSHAPE;
+  if (!x || (q != nullptr) != (s != nullptr) || (qt != nullptr) != (st != nullptr) ||
+      (!q && !qt))
+    return ACC_EBADARG;
+  if (sum && (!ws || ws_elems < accunet_fp8_sum_ws_elems(R, C))) return ACC_EBADARG;
+  const int CP = (int)fp8_pad(C), SP = (int)fp8_scale_pitch(C);
+  const long RP = fp8_pad(R);
+  const int SPT = (int)fp8_scale_pitch(R);
+  hipStream_t str = (hipStream_t)stream;
+  const int rc = with_dt(dt, [&](auto tag) {
+    using T = decltype(tag);
+    // 16-byte loads of 4 (fp32) or 8-byte loads of 4 (bf16)
+    const int vec = C % 4 == 0 && ((uintptr_t)x & (4 * sizeof(T) - 1)) == 0;
+    if (!square && !qt && !sum) {
+      const long n = R * SP * 16;
+      hipLaunchKernelGGL(fp8_rows_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, str,
+                         (const T*)x, (unsigned char*)q, (unsigned char*)s, R, C, CP, SP, vec);
+      return;
+    }
+    hipLaunchKernelGGL(fp8_tile_kernel<T>, dim3((unsigned)(RP / 128), CP / 128), dim3(256), 0, str,
+                       (const T*)x, (unsigned char*)q, (unsigned char*)s, (unsigned char*)qt,
+                       (unsigned char*)st, sum ? ws : nullptr, R, C, CP, SP, RP, SPT, square, vec);
+    if (sum)
+      hipLaunchKernelGGL(fp8_colsum_kernel, dim3(ceil_div(C, 64)), dim3(256), 0, str, ws, RP / 128,
+                         C, sum);
+  });
+  if (rc != ACC_OK) return rc;
+  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
+}

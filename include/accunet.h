@@ -552,6 +552,30 @@ int accunet_distill_planes_bwd(const void* z, const int* id, const float* p, con
                                long S, int V, int K, float T, float weight, int dt, void* stream);
 int accunet_distill_loss(const double* part, long n, const int* count, float* out, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * 8-bit linear layer: e4m3 values with a power-of-two scale for each block of 128 along the
+ * contracted axis (a third GEMM engine beside fp32 and bf16; no reference counterpart).
+ * A quantised matrix [R][C]: q [R][CP] bytes, CP = C rounded up to 128 (zeros behind C), and
+ * s [R][SP] bytes, byte j the biased exponent (e + 127) of the scale 2^e of columns
+ * [128 j, 128 j + 128), SP = CP / 128 rounded up to 4 (padding 127). e is the least integer
+ * with amax <= 448 * 2^e over the block's finite elements, in [-126, 120]; 0 for zeros.
+ *   accunet_fp8_quantize: x [R][C] of storage dt -> q, s with blocks 1 x 128 (128 x 128
+ *     with square, the byte repeated over the rows), and / or qt, st: the transposed matrix
+ *     [C][R] with blocks along R (square: the same blocks). sum (fp32 [C], or NULL): the
+ *     column sums of x, through ws of accunet_fp8_sum_ws_elems fp32 elements.
+ *   accunet_fp8_gemm: c [M][N] (storage cdt) = A B^T (+ bias fp32 [N]) of quantised A [M][K]
+ *     and B [N][K], fp32 accumulation; ws: accunet_fp8_gemm_ws_elems fp32 elements.
+ * q, qt: 16-byte aligned; s, st: 4-byte aligned.
+ * ------------------------------------------------------------------------- */
+size_t accunet_fp8_sum_ws_elems(long R, int C);
+int accunet_fp8_quantize(const void* x, int square, void* q, void* s, void* qt, void* st,
+                         float* sum, float* ws, size_t ws_elems, long R, int C, int dt,
+                         void* stream);
+size_t accunet_fp8_gemm_ws_elems(long M, long N, long K);
+int accunet_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb,
+                     const float* bias, void* c, float* ws, size_t ws_elems, long M, long N, long K,
+                     int cdt, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
