@@ -589,16 +589,36 @@ def subsample2(src, dst, B, H, W, C, bwd):
     call("accunet_subsample2", _p(src), _p(dst), B, H, W, C, int(bwd), _stream())
 
 
-# --------------------------------------------------- norms around a residual block
+# ------------------------------------------------------------------ token-block kernels
+# These calls are short, so their host path is too: pointers go as plain integers, and the
+# stream is torch's raw handle (the Stream object of `_stream` costs 3-5 us a call).
+def _a(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call_on(tensors, name, *args):
+    """Call `name` with `args` and the current stream of the tensors' device (they must share
+    one), which is made the current device for the launch if it is not."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise _lib.AccError(f"{name}: tensors on {tensors[0].device} and {t.device}")
+    if dev == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+# norms around a residual block
 def blocknorm_fwd(x, f, w1, b1, s, g, w2, b2, layer, eps, r, h, stats, P, L, C):
     """r, h (and stats, for a backward) of csrc/blocknorm.h; a gate of one row per sample
     has L rows a sample, of one row per token L = 1."""
     if P == 0:
         return
-    with _on(x, f, w1, b1, s, g, w2, b2):
-        call("accunet_blocknorm_fwd", _p(x), _p(f), _p(w1), _p(b1), _p(s), _p(g),
-             _gate_mode(g, L), _p(w2), _p(b2), 1 if layer else 0, eps, _p(r), _p(h), _p(stats),
-             P, L, C, _dt(x), _stream())
+    _call_on((x, f, w1, b1, s, g, w2, b2), "accunet_blocknorm_fwd", _a(x), _a(f), _a(w1), _a(b1),
+             _a(s), _a(g), _gate_mode(g, L), _a(w2), _a(b2), 1 if layer else 0, eps, _a(r), _a(h),
+             _a(stats), P, L, C, _dt(x))
 
 
 def blocknorm_bwd(x, f, w1, b1, s, g, w2, layer, stats, dr, dh, dx, df, dg, dpar, P, L, C):
@@ -607,87 +627,58 @@ def blocknorm_bwd(x, f, w1, b1, s, g, w2, layer, stats, dr, dh, dx, df, dg, dpar
         if dg is not None:
             dg.zero_()
         return
-    with _on(x, f, w1, b1, s, g, w2, dr, dh):
-        mode = _gate_mode(g, L)
-        n = int(_lib.load().accunet_blocknorm_ws_elems(P, L, C, mode))
-        ws = workspace(n, x.device)
-        call("accunet_blocknorm_bwd", _p(x), _p(f), _p(w1), _p(b1), _p(s), _p(g), mode, _p(w2),
-             1 if layer else 0, _p(stats), _p(dr), _p(dh), _p(dx), _p(df), _p(dg), _p(dpar),
-             _p(ws), n, P, L, C, _dt(x), _stream())
+    mode = _gate_mode(g, L)
+    n = int(_lib.load().accunet_blocknorm_ws_elems(P, L, C, mode))
+    ws = workspace(n, x.device)
+    _call_on((x, dr, dh), "accunet_blocknorm_bwd", _a(x), _a(f), _a(w1), _a(b1), _a(s), _a(g), mode,
+             _a(w2), 1 if layer else 0, _a(stats), _a(dr), _a(dh), _a(dx), _a(df), _a(dg), _a(dpar),
+             _a(ws), n, P, L, C, _dt(x))
 
 
 def _gate_mode(g, L) -> int:
     return 0 if g is None else (2 if L == 1 else 1)
 
 
-class _on:
-    """The device of the given tensors made the current one (they must share it), so the
-    launch and its stream are that device's whatever the caller's current device is."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, first, *rest):
-        dev = first.device
-        for t in rest:
-            if t is not None and t.device != dev:
-                raise _lib.AccError(f"tensors on {dev} and {t.device}")
-        self.guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-# --------------------------------------- distillation from a teacher's top logits
+# distillation from a teacher's top logits
 def distill_teacher(idx, top, rest, id_, p, tea, count, B, S, V, K, T):
-    with _on(idx, top, rest):
-        call("accunet_distill_teacher", _p(idx), 1 if idx.dtype == torch.int64 else 0, _p(top),
-             _dt(top), _p(rest), _p(id_), _p(p), _p(tea), _p(count), B, S, V, K, T, _stream())
+    _call_on((idx, top, rest), "accunet_distill_teacher", _a(idx),
+             1 if idx.dtype == torch.int64 else 0, _a(top), _dt(top), _a(rest), _a(id_), _a(p),
+             _a(tea), _a(count), B, S, V, K, T)
 
 
 def distill_fwd(z, rest, id_, p, tea, state, rowloss, part, B, S, V, K, T, weight, planes):
-    with _on(z, rest, id_):
-        if planes:
-            call("accunet_distill_planes_fwd", _p(z), _p(rest), _p(id_), _p(p), _p(tea),
-                 _p(state), _p(rowloss), _p(part), B, S, V, K, T, weight, _dt(z), _stream())
-            return
-        n = int(_lib.load().accunet_distill_rows_ws_elems(B, V, _dt(z)))
-        ws = workspace(n, z.device)
-        call("accunet_distill_rows_fwd", _p(z), _p(rest), _p(id_), _p(p), _p(tea), _p(state),
-             _p(rowloss), _p(part), _p(ws), n, B, V, K, T, weight, _dt(z), _stream())
+    if planes:
+        _call_on((z,), "accunet_distill_planes_fwd", _a(z), _a(rest), _a(id_), _a(p), _a(tea),
+                 _a(state), _a(rowloss), _a(part), B, S, V, K, T, weight, _dt(z))
+        return
+    n = int(_lib.load().accunet_distill_rows_ws_elems(B, V, _dt(z)))
+    ws = workspace(n, z.device)
+    _call_on((z,), "accunet_distill_rows_fwd", _a(z), _a(rest), _a(id_), _a(p), _a(tea), _a(state),
+             _a(rowloss), _a(part), _a(ws), n, B, V, K, T, weight, _dt(z))
 
 
 def distill_bwd(z, id_, p, state, up, up_rows, count, dz, B, S, V, K, T, weight, planes):
-    with _on(z, id_, up):
-        if planes:
-            call("accunet_distill_planes_bwd", _p(z), _p(id_), _p(p), _p(state), _p(up),
-                 1 if up_rows else 0, _p(count), _p(dz), B, S, V, K, T, weight, _dt(z), _stream())
-        else:
-            call("accunet_distill_rows_bwd", _p(z), _p(id_), _p(p), _p(state), _p(up),
-                 1 if up_rows else 0, _p(count), _p(dz), B, V, K, T, weight, _dt(z), _stream())
+    args = (_a(z), _a(id_), _a(p), _a(state), _a(up), 1 if up_rows else 0, _a(count), _a(dz))
+    if planes:
+        _call_on((z, up), "accunet_distill_planes_bwd", *args, B, S, V, K, T, weight, _dt(z))
+    else:
+        _call_on((z, up), "accunet_distill_rows_bwd", *args, B, V, K, T, weight, _dt(z))
 
 
 def distill_loss(part, n, count, out):
-    with _on(part):
-        call("accunet_distill_loss", _p(part), n, _p(count), _p(out), _stream())
+    _call_on((part,), "accunet_distill_loss", _a(part), n, _a(count), _a(out))
 
 
-# ------------------------------------------------------------- 8-bit linear layer
+# 8-bit linear layer
 def fp8_quantize(x, square, q, s, qt, st, sum_, R, C):
-    with _on(x):
-        n = int(_lib.load().accunet_fp8_sum_ws_elems(R, C)) if sum_ is not None else 0
-        ws = workspace(n, x.device) if n else None
-        call("accunet_fp8_quantize", _p(x), 1 if square else 0, _p(q), _p(s), _p(qt), _p(st),
-             _p(sum_), _p(ws), n, R, C, _dt(x), _stream())
+    n = int(_lib.load().accunet_fp8_sum_ws_elems(R, C)) if sum_ is not None else 0
+    ws = workspace(n, x.device) if n else None
+    _call_on((x,), "accunet_fp8_quantize", _a(x), 1 if square else 0, _a(q), _a(s), _a(qt), _a(st),
+             _a(sum_), _a(ws), n, R, C, _dt(x))
 
 
 def fp8_gemm(a, sa, b, sb, bias, c, M, N, K):
-    with _on(a, sa, b, sb, bias, c):
-        n = int(_lib.load().accunet_fp8_gemm_ws_elems(M, N, K))
-        ws = workspace(n, a.device) if n else None
-        call("accunet_fp8_gemm", _p(a), _p(sa), _p(b), _p(sb), _p(bias), _p(c), _p(ws), n, M, N, K,
-             _dt(c), _stream())
+    n = int(_lib.load().accunet_fp8_gemm_ws_elems(M, N, K))
+    ws = workspace(n, a.device) if n else None
+    _call_on((a, b, bias), "accunet_fp8_gemm", _a(a), _a(sa), _a(b), _a(sb), _a(bias), _a(c),
+             _a(ws), n, M, N, K, _dt(c))
