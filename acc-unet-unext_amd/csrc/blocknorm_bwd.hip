@@ -12,77 +12,78 @@
 // dw2, db2) hold every parameter gradient. Each block writes its sums once; finish kernels
 // add the blocks' rows in a fixed order (no atomics).
 // Bound by memory: x, f, dr, dh read once, dx, df written once (an element gate adds one
-// read and one write).
+// read and one write). Per-channel sums and parameters take 56 registers a thread, so a
+// row's threads are few enough for 2-3 waves a SIMD and the next row's loads are issued a
+// row ahead (327 -> 245 us at 16384 x 4096 bf16; parameters read 16 bytes at a time 194 us;
+// one block a CU and streaming stores 171 us, 4.7 TB/s).
 #include "blocknorm.h"
 
-template <typename T, int VEC, int ITER, int WPR, bool POST>
+// ge: the gate has a row of its own for every token
+template <typename T, int ITER, int WPR, int FORM, bool POST, bool ge>
 __global__ void __launch_bounds__(WPR == 1 ? 256 : 64 * WPR)
 blocknorm_bwd_kernel(const BlockNormArgs a) {
+  constexpr int N = BnGroup<T>::N, NE = ITER * N;
   constexpr int RT = 64 * WPR;
   constexpr int RPB = WPR == 1 ? 4 : 1;
-  constexpr int NE = ITER * VEC;
+  constexpr bool AHEAD = WPR < 16;  // 16 waves leave too few registers for the next row
   __shared__ float red[2][2][16];
   __shared__ float fold[WPR == 1 ? 4 : 1][2][WPR == 1 ? NE * 64 : 1];
+  // sum g*A, sum g*B over the samples of the block; each thread owns its columns
+  __shared__ float tot[POST ? 2 : 1][POST ? NE * RT : 1];
   int turn = 0;
   const int t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const int sub = WPR == 1 ? (threadIdx.x >> 6) : 0;
+  const int sub = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int C = a.C;
   const float inv = 1.f / (float)C;
-  const float layer = a.layer ? 1.f : 0.f;
-  const bool gs = a.gmode == BN_GATE_SAMPLE, ge = a.gmode == BN_GATE_ELEMENT;
-  float w1[NE], b1[NE], s[NE], w2[NE], g[NE];
-  float A[NE], B[NE], gA[NE], gB[NE], D[NE], E[NE];
-  int col[ITER];
-  bool on[ITER];
-  auto each = [&](auto fn) {
-#pragma unroll
-    for (int i = 0; i < ITER; ++i)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) fn(i, i * VEC + j, j);
-  };
+  const float layer = a.layer ? inv : 0.f;
+  const bool gs = a.gmode == BN_GATE_SAMPLE;
+  // s*w1 and s*b1, times the gate of a sample (an element gate multiplies later), and w2
+  float p1[NE], p0[NE], w2[NE];
+  float A[NE], B[NE], D[NE], E[NE];
+  int col[ITER], n[ITER];
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
-    col[i] = (i * RT + t) * VEC;
-    on[i] = col[i] < C;
-    if (!on[i]) col[i] = 0;
+    const int c = (i * RT + t) * N;
+    n[i] = max(0, min(N, C - c));
+    col[i] = n[i] > 0 ? c : 0;
   }
-  each([&](int i, int k, int j) {
-    if (POST) {
-      w1[k] = a.w1 ? a.w1[col[i] + j] : 1.f;
-      b1[k] = a.b1 ? a.b1[col[i] + j] : 0.f;
-      s[k] = a.s ? a.s[col[i] + j] : 1.f;
-      gA[k] = gB[k] = 0.f;
-    }
-    w2[k] = a.w2 ? a.w2[col[i] + j] : 1.f;
-    D[k] = E[k] = 0.f;
-    g[k] = 1.f;
-  });
-  const T* X = (const T*)a.x;
-  const T* F = (const T*)a.f;
-  const T* Gt = (const T*)a.g;
-  const T* DR = (const T*)a.dr;
-  const T* DH = (const T*)a.dh;
-  auto load = [&](const T* base, long p, float* v) {
+  auto each = [&](auto fn) {
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      float q[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) q[j] = 0.f;
-      if (on[i]) bn_load<VEC>(base + p * C + col[i], q);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = q[j];
-    }
+    for (int k = 0; k < NE; ++k) fn(k, k % N < n[k / N], k % N < n[k / N] ? col[k / N] + k % N : 0);
   };
-  auto store = [&](T* base, long p, const float* v) {
+  auto par = [&](const float* p, float fill, float* v) {
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      float q[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) q[j] = v[i * VEC + j];
-      if (on[i]) bn_store<VEC>(base + p * C + col[i], q);
-    }
+    for (int i = 0; i < ITER; ++i)
+      bn_params<N>(p ? p + col[i] : nullptr, n[i], fill, v + i * N);
   };
-  // u, v: the sums of this block over its waves, left in wave 0 (WPR == 1)
+  par(a.w2, 1.f, w2);
+  // p1, p0 = m * w1, m * b1
+  auto products = [&](const float* m) {
+    par(a.w1, 1.f, p1);
+    par(a.b1, 0.f, p0);
+    each([&](int k, bool, int) {
+      p1[k] *= m[k];
+      p0[k] *= m[k];
+    });
+  };
+  each([&](int k, bool, int) { D[k] = E[k] = 0.f; });
+  if (POST) {
+    float m[NE];
+    par(a.s, 1.f, m);
+    products(m);
+    if (sub == 0) each([&](int k, bool, int) { tot[0][k * RT + t] = tot[1][k * RT + t] = 0.f; });
+  }
+  auto load = [&](const void* base, long row, BnGroup<T> (&g)[ITER]) {
+    const T* p = (const T*)base + row * C;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) g[i] = bn_load<T, FORM>(p + col[i], n[i]);
+  };
+  auto store = [&](void* base, long row, const float* v) {
+    T* p = (T*)base + row * C;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) bn_store<T, FORM>(p + col[i], n[i], v + i * N);
+  };
+  // u, v: the sums of this block over its waves, in every wave (WPR == 1)
   auto fold_waves = [&](float* u, float* v) {
     if constexpr (WPR == 1) {
       __syncthreads();
@@ -110,32 +111,52 @@ blocknorm_bwd_kernel(const BlockNormArgs a) {
   const long s1 = min(nb, s0 + (a.S > 1 ? 1 : a.G));
   const int part = a.S > 1 ? blockIdx.x % a.S : 0;
   const long chunk = (a.L + a.S - 1) / a.S;
+  BnGroup<T> nx[ITER], nf[ITER], nd[ITER], nh[ITER], ng[ITER];
+  float4 nst;
+  auto fetch = [&](long p) {
+    nst = ld4(a.stats + 4 * p);
+    load(a.x, p, nx);
+    if (POST) load(a.f, p, nf);
+    if (a.dh) load(a.dh, p, nh);
+    if (a.dr) load(a.dr, p, nd);
+    if (POST && ge) load(a.g, p, ng);
+  };
   for (long smp = s0; smp < s1; ++smp) {
     if (POST) {
-      if (gs) load(Gt, smp, g);
+      if (gs) {
+        float m[NE];
+        par(a.s, 1.f, m);
+        load(a.g, smp, ng);
+        each([&](int k, bool, int) { m[k] *= ng[k / N].get(k % N); });
+        products(m);
+      }
 #pragma unroll
       for (int k = 0; k < NE; ++k) A[k] = B[k] = 0.f;
     }
     const long r0 = smp * a.L + part * chunk, r1 = min((smp + 1) * a.L, r0 + chunk);
+    if (AHEAD && r0 + sub < r1) fetch(r0 + sub);
     for (long p = r0 + sub; p < r1; p += RPB) {
-      const float4 st = ld4(a.stats + 4 * p);
-      float x[NE], f[NE], d[NE], h[NE];
-      load(X, p, x);
-      if (POST) load(F, p, f);
-      if (a.dh) load(DH, p, h);
-      if (a.dr) load(DR, p, d);
-      if (POST) {
-        if (ge) load(Gt, p, g);
-        each([&](int i, int k, int) {
-          f[k] = on[i] ? (f[k] - st.x) * st.y : 0.f;
-          x[k] += s[k] * g[k] * (f[k] * w1[k] + b1[k]);
-        });
+      if (!AHEAD) fetch(p);
+      const float4 st = nst;
+      float x[NE], f[NE], d[NE], h[NE], g[NE];
+#pragma unroll
+      for (int k = 0; k < NE; ++k) {
+        x[k] = nx[k / N].get(k % N);
+        if (POST) f[k] = nf[k / N].get(k % N);
+        h[k] = a.dh ? nh[k / N].get(k % N) : 0.f;
+        d[k] = a.dr ? nd[k / N].get(k % N) : 0.f;
+        g[k] = POST && ge ? ng[k / N].get(k % N) : 1.f;
       }
-      if (!a.dr) each([&](int, int k, int) { d[k] = 0.f; });
+      if (AHEAD && p + RPB < r1) fetch(p + RPB);
+      if (POST)
+        each([&](int k, bool on, int) {
+          f[k] = on ? (f[k] - st.x) * st.y : 0.f;
+          x[k] += g[k] * (f[k] * p1[k] + p0[k]);
+        });
       if (a.dh) {
         float q[2] = {0.f, 0.f};
-        each([&](int i, int k, int) {
-          x[k] = on[i] ? (x[k] - st.z) * st.w : 0.f;  // rhat
+        each([&](int k, bool on, int) {
+          x[k] = on ? (x[k] - st.z) * st.w : 0.f;  // rhat
           D[k] += h[k] * x[k];
           E[k] += h[k];
           h[k] *= w2[k];
@@ -143,45 +164,51 @@ blocknorm_bwd_kernel(const BlockNormArgs a) {
           q[1] += h[k] * x[k];
         });
         bn_row_sum<WPR, 2>(q, red, turn);
-        const float m0 = layer * q[0] * inv, m1 = q[1] * inv;
-        each([&](int, int k, int) { d[k] += st.w * (h[k] - m0 - x[k] * m1); });
+        const float m0 = layer * q[0], m1 = q[1] * inv;
+        each([&](int k, bool on, int) {
+          d[k] = on ? d[k] + st.w * (h[k] - m0 - x[k] * m1) : 0.f;
+        });
       }
-      store((T*)a.dx, p, d);
+      store(a.dx, p, d);
       if (POST) {
         float q[2] = {0.f, 0.f};
-        each([&](int i, int k, int) {
-          if (!on[i]) d[k] = 0.f;
-          const float dg = ge ? d[k] * g[k] : d[k];
+        each([&](int k, bool, int) {
+          const float dg = d[k] * g[k];
           A[k] += dg * f[k];
           B[k] += dg;
-          h[k] = d[k] * s[k] * g[k] * w1[k];
+          h[k] = dg * p1[k];
           q[0] += h[k];
           q[1] += h[k] * f[k];
-          if (ge) d[k] *= s[k] * (f[k] * w1[k] + b1[k]);
+          if (ge) d[k] *= f[k] * p1[k] + p0[k];  // the gate's gradient
         });
-        if (ge && a.dg) store((T*)a.dg, p, d);
+        if (ge) store(a.dg, p, d);
         bn_row_sum<WPR, 2>(q, red, turn);
-        const float m0 = layer * q[0] * inv, m1 = q[1] * inv;
-        each([&](int, int k, int) { h[k] = st.y * (h[k] - m0 - f[k] * m1); });
-        store((T*)a.df, p, h);
+        const float m0 = layer * q[0], m1 = q[1] * inv;
+        each([&](int k, bool, int) { h[k] = st.y * (h[k] - m0 - f[k] * m1); });
+        store(a.df, p, h);
       }
     }
     if (POST) {
       fold_waves(A, B);
-      each([&](int, int k, int) {
-        gA[k] += gs ? g[k] * A[k] : A[k];
-        gB[k] += gs ? g[k] * B[k] : B[k];
-        A[k] = s[k] * (w1[k] * A[k] + b1[k] * B[k]);
-      });
-      if (gs && sub == 0) {
-        if (a.S == 1) {
-          store((T*)a.dg, smp, A);
-        } else {
+      if (gs) load(a.g, smp, ng);
+      if (sub == 0) {
+        each([&](int k, bool, int) {
+          const float gk = gs ? ng[k / N].get(k % N) : 1.f;
+          tot[0][k * RT + t] += gk * A[k];
+          tot[1][k * RT + t] += gk * B[k];
+        });
+        if (gs) {  // dg = s * (w1 * A + b1 * B)
+          float m[NE];
+          par(a.s, 1.f, m);
+          products(m);
+          each([&](int k, bool, int) { A[k] = p1[k] * A[k] + p0[k] * B[k]; });
+          if (a.S == 1) {
+            store(a.dg, smp, A);
+          } else {
 #pragma unroll
-          for (int i = 0; i < ITER; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-              if (on[i]) a.gpart[(long)blockIdx.x * C + col[i] + j] = A[i * VEC + j];
+            for (int i = 0; i < ITER; ++i)
+              bn_put<N>(a.gpart + (long)blockIdx.x * C + col[i], n[i], A + i * N);
+          }
         }
       }
     }
@@ -189,16 +216,19 @@ blocknorm_bwd_kernel(const BlockNormArgs a) {
   fold_waves(D, E);
   if (sub == 0) {
     float* o = a.part + (long)blockIdx.x * 4 * C;
-    each([&](int i, int k, int j) {
-      if (!on[i]) return;
-      const int c = col[i] + j;
+    if (POST) each([&](int k, bool, int) {
+        A[k] = tot[0][k * RT + t];
+        B[k] = tot[1][k * RT + t];
+      });
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
       if (POST) {
-        o[c] = gA[k];
-        o[C + c] = gB[k];
+        bn_put<N>(o + col[i], n[i], A + i * N);
+        bn_put<N>(o + C + col[i], n[i], B + i * N);
       }
-      o[2 * C + c] = D[k];
-      o[3 * C + c] = E[k];
-    });
+      bn_put<N>(o + 2 * C + col[i], n[i], D + i * N);
+      bn_put<N>(o + 3 * C + col[i], n[i], E + i * N);
+    }
   }
 }
 
@@ -265,7 +295,10 @@ static BnPlan bn_plan(long P, long L, int C, int gmode) {
   q.gmode = gmode == BN_GATE_SAMPLE && L == 1 ? BN_GATE_ELEMENT : gmode;
   q.L = q.gmode == BN_GATE_SAMPLE ? L : P;
   const int rpb = C <= 512 ? 4 : 1;
-  const long want = C <= 1024 ? 1024 : C <= 2048 ? 768 : C <= 4096 ? 512 : 256;
+  // blocks that fill the card once: one a CU from 513 threads on, more of the smaller ones;
+  // every block writes a row of partial sums, so more of them cost traffic (C = 4096: 512
+  // blocks 194 us for 16384 bf16 rows, 256 blocks 174 us)
+  const long want = C <= 1024 ? 1024 : C <= 2048 ? 768 : 256;
   const long n = P / q.L;
   q.G = n >= want ? (int)((n + want - 1) / want) : 1;
   q.S = n >= want ? 1 : (int)min((want + n - 1) / n, (q.L + rpb - 1) / rpb);
@@ -303,20 +336,21 @@ extern "C" int accunet_blocknorm_bwd(const void* x, const void* f, const float* 
   a.gpart = ws + (size_t)q.blocks * 4 * C;
   a.P = P; a.L = q.L; a.C = C; a.gmode = q.gmode; a.layer = layer != 0;
   a.G = q.G; a.S = q.S;
-  const bool vec = bn_aligned(x) && bn_aligned(f) && bn_aligned(g) && bn_aligned(dr) &&
-                   bn_aligned(dh) && bn_aligned(dx) && bn_aligned(df) && bn_aligned(dg);
+  const bool aligned = bn_aligned(x) && bn_aligned(f) && bn_aligned(g) && bn_aligned(dr) &&
+                    bn_aligned(dh) && bn_aligned(dx) && bn_aligned(df) && bn_aligned(dg);
   hipStream_t st = (hipStream_t)stream;
   with_dt(dt, [&](auto tag) {
     using T = decltype(tag);
-    bn_with_shape<T>(C, vec, [&](auto sh) {
+    bn_with_shape<T>(P, C, aligned, [&](auto sh) {
       using Sh = decltype(sh);
       const int nth = Sh::WPR == 1 ? 256 : 64 * Sh::WPR;
-      if (f)
-        hipLaunchKernelGGL((blocknorm_bwd_kernel<T, Sh::VEC, Sh::ITER, Sh::WPR, true>),
-                           dim3(q.blocks), dim3(nth), 0, st, a);
-      else
-        hipLaunchKernelGGL((blocknorm_bwd_kernel<T, Sh::VEC, Sh::ITER, Sh::WPR, false>),
-                           dim3(q.blocks), dim3(nth), 0, st, a);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(q.blocks), dim3(nth), 0, st, a);
+      };
+      if (!f) go(blocknorm_bwd_kernel<T, Sh::ITER, Sh::WPR, Sh::FORM, false, false>);
+      else if (q.gmode == BN_GATE_ELEMENT)
+        go(blocknorm_bwd_kernel<T, Sh::ITER, Sh::WPR, Sh::FORM, true, true>);
+      else go(blocknorm_bwd_kernel<T, Sh::ITER, Sh::WPR, Sh::FORM, true, false>);
     });
     if (q.gmode == BN_GATE_SAMPLE && q.S > 1) {
       const long n = P / L * C;
