@@ -24,50 +24,44 @@ from ._lib import AccError
 
 MAX_K = 256
 _PLANES_MAX_V = 1024
-_REDUCTIONS = ("mean", "sum", "none")
+_REDUCTIONS = ("none", "sum", "mean")
+
+
+def _forward(z, idx, top, rest, T, weight, reduction, B, S, V, K, dz):
+    n = B * S
+    none = reduction == 0
+    if n == 0:
+        return torch.zeros((0,) if none else (), dtype=torch.float32, device=z.device), None
+    loss = torch.empty((n,) if none else (), dtype=torch.float32, device=z.device)
+    return loss, kern.distill_fwd(z, idx, top, rest, loss, reduction, dz, B, S, V, K, T, weight)
 
 
 class _DistillFn(torch.autograd.Function):
+    """The forward writes the gradient for an upstream of 1 where one kernel can do both
+    (sum and mean), and the backward hands that tensor out, once: its kernel rewrites it only
+    for another upstream gradient. A further backward of the same graph computes it anew."""
+
     @staticmethod
-    def forward(ctx, z, idx, top, rest, T, weight, reduction, B, S, V, K, planes):
-        dev = z.device
-        n = B * S
-        f32 = torch.float32
-        none = reduction == "none"
-        if n == 0:
-            ctx.empty = True
-            ctx.like = z.shape, z.dtype
-            return torch.zeros((0,) if none else (), dtype=f32, device=dev)
-        ctx.empty = False
-        id_ = torch.empty(n * K, dtype=torch.int32, device=dev)
-        p = torch.empty(n * K, dtype=f32, device=dev)
-        tea = torch.empty(n, 2, dtype=f32, device=dev)
-        state = torch.empty(n, 4, dtype=f32, device=dev)
-        count = torch.zeros(1, dtype=torch.int32, device=dev)
-        kern.distill_teacher(idx, top, rest, id_, p, tea, count, B, S, V, K, T)
-        rowloss = torch.empty(n, dtype=f32, device=dev) if none else None
-        nb = (n + 255) // 256 if planes else n
-        part = torch.empty(nb, dtype=torch.float64, device=dev)
-        kern.distill_fwd(z, rest, id_, p, tea, state, rowloss, part, B, S, V, K, T, weight, planes)
-        if not none:
-            loss = torch.empty((), dtype=f32, device=dev)
-            kern.distill_loss(part, nb, count if reduction == "mean" else None, loss)
-        ctx.save_for_backward(z, id_, p, state, count)
-        ctx.cfg = (T, weight, reduction, B, S, V, K, planes)
-        return rowloss if none else loss
+    def forward(ctx, z, idx, top, rest, T, weight, reduction, B, S, V, K):
+        fuse = reduction != 0 and B * S > 0 and kern.distill_fused(B, S, V, kern._dt(z))
+        ctx.dz = torch.empty_like(z) if fuse else None
+        loss, save = _forward(z, idx, top, rest, T, weight, reduction, B, S, V, K, ctx.dz)
+        ctx.save_for_backward(z, save)
+        ctx.cfg = (reduction, B, S, V, K, T, weight)
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        if ctx.empty:
-            shape, dtype = ctx.like
-            return (torch.zeros(shape, dtype=dtype, device=up.device),) + (None,) * 11
-        z, id_, p, state, count = ctx.saved_tensors
-        T, weight, reduction, B, S, V, K, planes = ctx.cfg
-        dz = torch.empty_like(z)
-        kern.distill_bwd(z, id_, p, state, up.contiguous(), reduction == "none",
-                         count if reduction == "mean" else None, dz, B, S, V, K, T, weight, planes)
-        return (dz,) + (None,) * 11
+        z, save = ctx.saved_tensors
+        dz, ctx.dz = ctx.dz, None
+        held = dz is not None
+        if not held:
+            dz = torch.empty_like(z)
+        if save is not None:
+            reduction, B, S, V, K, T, weight = ctx.cfg
+            kern.distill_bwd(z, save, up.contiguous(), reduction, held, dz, B, S, V, K, T, weight)
+        return (dz,) + (None,) * 10
 
 
 def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight=1.0,
@@ -78,7 +72,8 @@ def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight
     int64) and top_logits (float32 or bfloat16): the same shape with K <= 256 entries in
     place of the V classes. rest: float32, the shape without that axis, in [0, 1].
     reduction: "mean" over the rows that have an entry, "sum", or "none" (one loss a row).
-    `weight` multiplies the loss. Non-contiguous inputs are copied, and so are more than
+    `weight` multiplies the loss (inside: a factor applied to the result, 0.5 * loss, costs the
+    backward another pass over the logits). Non-contiguous inputs are copied, and so are more than
     1024 classes on dim=1."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
@@ -126,7 +121,11 @@ def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight
     z = logits.contiguous()
     if z.data_ptr() % 16:
         z = z.clone()
-    loss = _DistillFn.apply(z, top_idx.contiguous(), top_logits.contiguous(),
-                            rest.contiguous() if rest is not None else None, temperature, weight,
-                            reduction, B, S if planes else 1, V, K, planes)
+    args = (z, top_idx.contiguous(), top_logits.contiguous(),
+            rest.contiguous() if rest is not None else None, temperature, weight,
+            _REDUCTIONS.index(reduction), B, S if planes else 1, V, K)
+    if z.requires_grad and torch.is_grad_enabled():
+        loss = _DistillFn.apply(*args)
+    else:
+        loss = _forward(*args, None)[0]
     return loss.view(outer) if reduction == "none" else loss

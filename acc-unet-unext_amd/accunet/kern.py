@@ -640,33 +640,26 @@ def _gate_mode(g, L) -> int:
 
 
 # distillation from a teacher's top logits
-def distill_teacher(idx, top, rest, id_, p, tea, count, B, S, V, K, T):
-    _call_on((idx, top, rest), "accunet_distill_teacher", _a(idx),
-             1 if idx.dtype == torch.int64 else 0, _a(top), _dt(top), _a(rest), _a(id_), _a(p),
-             _a(tea), _a(count), B, S, V, K, T)
+def distill_fused(B, S, V, dt) -> bool:
+    """Whether the forward can write the gradient in the same pass."""
+    return bool(_lib.load().accunet_distill_fused(B, S, V, dt))
 
 
-def distill_fwd(z, rest, id_, p, tea, state, rowloss, part, B, S, V, K, T, weight, planes):
-    if planes:
-        _call_on((z,), "accunet_distill_planes_fwd", _a(z), _a(rest), _a(id_), _a(p), _a(tea),
-                 _a(state), _a(rowloss), _a(part), B, S, V, K, T, weight, _dt(z))
-        return
-    n = int(_lib.load().accunet_distill_rows_ws_elems(B, V, _dt(z)))
-    ws = workspace(n, z.device)
-    _call_on((z,), "accunet_distill_rows_fwd", _a(z), _a(rest), _a(id_), _a(p), _a(tea), _a(state),
-             _a(rowloss), _a(part), _a(ws), n, B, V, K, T, weight, _dt(z))
+def distill_fwd(z, idx, top, rest, loss, reduction, dz, B, S, V, K, T, weight):
+    """The loss (and dz for an upstream of 1, where given); returns what a backward needs."""
+    lib, dt = _lib.load(), _dt(z)
+    n, m = lib.accunet_distill_save_bytes(B, S, V, K), lib.accunet_distill_ws_bytes(B, S, V, K, dt)
+    save = torch.empty(n, dtype=torch.uint8, device=z.device)
+    ws = torch.empty(m, dtype=torch.uint8, device=z.device)
+    _call_on((z, idx, top, rest), "accunet_distill_fwd", _a(z), _a(idx),
+             1 if idx.dtype == torch.int64 else 0, _a(top), _dt(top), _a(rest), _a(loss), reduction,
+             _a(dz), _a(save), n, _a(ws), m, B, S, V, K, T, weight, dt)
+    return save
 
 
-def distill_bwd(z, id_, p, state, up, up_rows, count, dz, B, S, V, K, T, weight, planes):
-    args = (_a(z), _a(id_), _a(p), _a(state), _a(up), 1 if up_rows else 0, _a(count), _a(dz))
-    if planes:
-        _call_on((z, up), "accunet_distill_planes_bwd", *args, B, S, V, K, T, weight, _dt(z))
-    else:
-        _call_on((z, up), "accunet_distill_rows_bwd", *args, B, V, K, T, weight, _dt(z))
-
-
-def distill_loss(part, n, count, out):
-    _call_on((part,), "accunet_distill_loss", _a(part), n, _a(count), _a(out))
+def distill_bwd(z, save, up, reduction, held, dz, B, S, V, K, T, weight):
+    _call_on((z, up), "accunet_distill_bwd", _a(z), _a(save), save.numel(), _a(up), reduction,
+             1 if held else 0, _a(dz), B, S, V, K, T, weight, _dt(z))
 
 
 # 8-bit linear layer

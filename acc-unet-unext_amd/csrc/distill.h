@@ -61,6 +61,9 @@ ACC_DEV void dt_wave_join(float& m, float& s, float c) {
     const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
     dt_join(m, s, m2, s2, c);
   }
+  // partners round their joint sum differently: every lane takes the first lane's
+  m = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m)));
+  s = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(s)));
 }
 
 // The row's state and loss (base 2, before T^2 ln 2) once (m, s) over the streamed classes,
@@ -88,7 +91,7 @@ ACC_DEV DtRow dt_row_state(float m, float s, float mr, float sr, float rest, boo
 
 // the step from a row's sums to its gradient: weight * T * upstream / rows counted
 struct DtScale {
-  const float* up;      // upstream gradient: one value, or one per row (up_rows)
+  const float* up;      // upstream gradient: one value, or one per row (up_rows); null: 1
   int up_rows;
   const int* count;     // rows counted (mean), or null
   float k;              // weight * T
@@ -99,3 +102,32 @@ ACC_DEV float dt_scale(const DtScale& g, long row) {
   if (g.count) v /= (float)max(*g.count, 1);
   return v;
 }
+
+// One call's arguments. `rows` = B * S; S = 1 with the classes last.
+struct DtArgs {
+  const void* z;
+  const float* rest;
+  // kept for the backward
+  float4* state;      // [rows]
+  float* applied;     // upstream gradient that dz holds: [rows], or one a block of 256 pixels
+  int* count;         // rows counted
+  int* id;            // [rows][K]
+  float* p;           // [rows][K]
+  // scratch of the forward
+  float2* tea;        // [rows]
+  double* part;       // partial losses
+  int* cnt;           // rows counted by each block of the teacher's pass
+  float2* ms;         // [rows][runs]
+  float* loss;        // the loss, or one a row (none)
+  void* dz;
+  long rows, S;
+  int V, K;
+  float T, c, scale, weight;
+  int none, mean;
+};
+
+// rows with the classes last (distill_rows.hip); up to DTR_WAVE_V classes a wave has a row
+#define DTR_WAVE_V 2048
+int dt_rows_runs(long R, int V, int dt);
+void dt_rows_forward(const DtArgs& a, int dt, hipStream_t st);
+void dt_rows_backward(const DtArgs& a, const DtScale& g, int dt, hipStream_t st);

@@ -1,26 +1,29 @@
 // Distillation from a teacher's top logits; mathematics in distill.h. This file: the
 // teacher's pass, the loss over the rows, and the layout with the classes on the channel
 // axis of an image (z [B][V][S]). Rows with the classes last: distill_rows.hip.
+#include <type_traits>
+
 #include "distill.h"
 
 // ------------------------------------------------------------------ the teacher's entries
 // p and the entries that count, each class once: id = the class at its first entry (p the
 // sum over its entries), -1 elsewhere. tea[row] = (sum p log2 p + rest log2 rest, 1 or 0).
-// Also counts the rows that have an entry (integers: the order of the adds is immaterial).
+// cnt[block]: the rows of the block that have an entry.
 //
 // One wave a row, entries k = lane + 64 i. Bound by latency: K^2 / 64 comparisons a lane.
 template <typename IT, typename TT>
 __global__ void __launch_bounds__(256)
 distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ top,
                             const float* __restrict__ rest, int* __restrict__ id,
-                            float* __restrict__ p, float2* __restrict__ tea, int* count, long R,
-                            int V, int K, float c) {
+                            float* __restrict__ p, float2* __restrict__ tea, int* __restrict__ cnt,
+                            long R, int V, int K, float c) {
+  __shared__ int alive[4];
   __shared__ int sid[4][DT_MAX_K];
   __shared__ float sp[4][DT_MAX_K];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long row = blockIdx.x * 4L + wave;
-  if (row >= R) return;
-  const int NI = (K + 63) / 64;
+  const bool in = row < R;
+  const int NI = in ? (K + 63) / 64 : 0;
   int my[DT_MAX_K / 64];
   float a[DT_MAX_K / 64];
   float mx = -INFINITY;
@@ -48,7 +51,7 @@ distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ t
   for (int i = 0; i < DT_MAX_K / 64; ++i)
     if (my[i] >= 0) sum += dt_exp2(__builtin_fmaf(a[i], c, -ref));
   sum = dt_wave_sum(sum);
-  const float r = live && rest ? rest[row] : 0.f;
+  const float r = in && live && rest ? rest[row] : 0.f;
   const float keep = 1.f - r, lg = log2f(sum) - log2f(keep);
   float h = 0.f;
 #pragma unroll
@@ -80,9 +83,11 @@ distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ t
     p[row * K + k] = v;
   }
   if (lane == 0) {
-    tea[row] = make_float2(h, live ? 1.f : 0.f);
-    if (live) atomicAdd(count, 1);
+    if (in) tea[row] = make_float2(h, live ? 1.f : 0.f);
+    alive[wave] = in && live ? 1 : 0;
   }
+  __syncthreads();
+  if (threadIdx.x == 0) cnt[blockIdx.x] = alive[0] + alive[1] + alive[2] + alive[3];
 }
 
 // Classes on the channel axis: idx, top [B][K][S], one thread a pixel; the entries of a
@@ -91,7 +96,7 @@ template <typename IT, typename TT>
 __global__ void __launch_bounds__(256)
 distill_teacher_planes_kernel(const IT* __restrict__ idx, const TT* __restrict__ top,
                               const float* __restrict__ rest, int* __restrict__ id,
-                              float* __restrict__ p, float2* __restrict__ tea, int* count, long N,
+                              float* __restrict__ p, float2* __restrict__ tea, int* __restrict__ cnt, long N,
                               long S, int V, int K, float c) {
   const long row = blockIdx.x * 256L + threadIdx.x;
   bool live = false;
@@ -135,65 +140,84 @@ distill_teacher_planes_kernel(const IT* __restrict__ idx, const TT* __restrict__
     }
     tea[row] = make_float2(h, live ? 1.f : 0.f);
   }
-  const unsigned long long m = __ballot(live);
-  if ((threadIdx.x & 63) == 0 && m) atomicAdd(count, __popcll(m));
+  const int m = __syncthreads_count(live);
+  if (threadIdx.x == 0) cnt[blockIdx.x] = m;
 }
 
-extern "C" int accunet_distill_teacher(const void* idx, int idx64, const void* top, int top_dt,
-                                       const float* rest, int* id, float* p, float* tea, int* count,
-                                       long B, long S, int V, int K, float T, void* stream) {
-  if (B <= 0 || S <= 0 || V <= 0 || V > DT_MAX_V || K <= 0 || K > DT_MAX_K) return ACC_EBADSHAPE;
-  if (!idx || !top || !id || !p || !tea || !count || !(T > 0.f)) return ACC_EBADARG;
-  const float c = (float)(DT_LOG2E / T);
-  hipStream_t st = (hipStream_t)stream;
-  auto go = [&](auto itag) {
-    using IT = decltype(itag);
-    return with_dt(top_dt, [&](auto tag) {
-      using TT = decltype(tag);
-      if (S == 1)
-        hipLaunchKernelGGL((distill_teacher_rows_kernel<IT, TT>), dim3((unsigned)((B + 3) / 4)),
-                           dim3(256), 0, st, (const IT*)idx, (const TT*)top, rest, id, p,
-                           (float2*)tea, count, B, V, K, c);
-      else
-        hipLaunchKernelGGL((distill_teacher_planes_kernel<IT, TT>),
-                           dim3((unsigned)((B * S + 255) / 256)), dim3(256), 0, st, (const IT*)idx,
-                           (const TT*)top, rest, id, p, (float2*)tea, count, B * S, S, V, K, c);
-    });
-  };
-  const int rc = idx64 ? go((long long)0) : go((int)0);
-  if (rc != ACC_OK) return rc;
-  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
+// count = sum of the n values of cnt
+__global__ void __launch_bounds__(1024)
+distill_count_kernel(const int* __restrict__ cnt, int n, int* __restrict__ count) {
+  __shared__ int red[16];
+  int v = 0;
+  for (int i = threadIdx.x; i < n; i += 1024) v += cnt[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int t = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t += red[w];
+    *count = t;
+  }
 }
 
 // ------------------------------------------------------- classes on the channel axis
 // One thread a pixel, the classes four at a time (loads of one class are contiguous over
 // the pixels). Listed classes are marked in a bitmap of the thread's own in LDS.
 #define DTP_MAX_V 1024
+//
+// The gradient of a pixel: every class as not listed, then the listed ones over it.
+template <typename T>
+ACC_DEV void dtp_gradient(const T* zr, T* dr, long S, int V, int K, const int* id, const float* p,
+                          const float4& st, float c, float gs) {
+  const float cu = st.y * gs;
+  for (int j0 = 0; j0 < V; j0 += 4) {
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = j0 + u < V ? ld1(zr + (long)(j0 + u) * S) : 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (j0 + u < V) st1(dr + (long)(j0 + u) * S, dt_exp2(__builtin_fmaf(v[u], c, -st.x)) * cu);
+  }
+  for (int k = 0; k < K; ++k) {
+    const int j = id[k * S];
+    if (j >= 0)
+      st1(dr + (long)j * S, gs * (dt_exp2(__builtin_fmaf(ld1(zr + (long)j * S), c, -st.z)) * st.w -
+                                  p[k * S]));
+  }
+}
+template <typename T>
+ACC_DEV void dtp_zero(T* dr, long S, int V) {
+  for (int j = 0; j < V; ++j) st1(dr + (long)j * S, 0.f);
+}
+
+// dz (or null): the gradient for an upstream of 1 too, from the logits still in the cache
 template <typename T, bool REST>
 __global__ void __launch_bounds__(256)
-distill_planes_fwd_kernel(const T* __restrict__ z, const float* __restrict__ rest,
-                          const int* __restrict__ id, const float* __restrict__ p,
-                          const float2* __restrict__ tea, float4* __restrict__ state,
-                          float* __restrict__ rowloss, double* __restrict__ part, long N, long S,
-                          int V, int K, float c, float scale) {
+distill_planes_fwd_kernel(const DtArgs a, const DtScale g) {
   extern __shared__ unsigned mask[];  // [words][256], REST only
   __shared__ double red[4];
   const int t = threadIdx.x;
-  const long row = blockIdx.x * 256L + t;
+  const long row = blockIdx.x * 256L + t, S = a.S;
+  const int V = a.V, K = a.K;
+  const float c = a.c;
   float loss = 0.f;
-  if (row < N) {
+  if (row < a.rows) {
     const long b = row / S, s0 = row - b * S;
-    const float2 te = tea[row];
+    const T* zr = (const T*)a.z + b * V * S + s0;
+    T* dr = a.dz ? (T*)a.dz + b * V * S + s0 : nullptr;
+    const long kb = b * K * S + s0;
+    const float2 te = a.tea[row];
     if (te.y == 0.f) {
-      state[row] = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
+      a.state[row] = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
+      if (dr) dtp_zero(dr, S, V);
     } else {
-      const T* zr = z + b * V * S + s0;
-      const long kb = b * K * S + s0;
       if (REST) {
         const int words = (V + 31) / 32;
         for (int w = 0; w < words; ++w) mask[w * 256 + t] = 0u;
         for (int k = 0; k < K; ++k) {
-          const int j = id[kb + k * S];
+          const int j = a.id[kb + k * S];
           if (j >= 0) mask[(j >> 5) * 256 + t] |= 1u << (j & 31);
         }
       }
@@ -219,63 +243,53 @@ distill_planes_fwd_kernel(const T* __restrict__ z, const float* __restrict__ res
       const float mr = m, sr = s;
       if (REST)
         for (int k = 0; k < K; ++k) {
-          const int j = id[kb + k * S];
+          const int j = a.id[kb + k * S];
           if (j >= 0) dt_join(m, s, ld1(zr + (long)j * S), 1.f, c);
         }
-      const float r = REST ? rest[row] : 0.f;
+      const float r = REST ? a.rest[row] : 0.f;
       const DtRow o = dt_row_state(m, s, mr, sr, r, REST, c);
       float dot = 0.f;
       for (int k = 0; k < K; ++k) {
-        const int j = id[kb + k * S];
-        const float pk = p[kb + k * S];
+        const int j = a.id[kb + k * S];
+        const float pk = a.p[kb + k * S];
         if (j >= 0 && !(pk == 0.f))
           dot += pk * (__builtin_fmaf(ld1(zr + (long)j * S), c, -o.M) - o.log2S);
       }
       if (REST && !(r == 0.f)) dot += r * ((dt_ref(mr, c) - o.M) + log2f(sr) - o.log2S);
-      state[row] = o.state;
-      loss = scale * (te.x - dot);
+      a.state[row] = o.state;
+      loss = a.scale * (te.x - dot);
+      if (dr) dtp_gradient(zr, dr, S, V, K, a.id + kb, a.p + kb, o.state, c, dt_scale(g, row));
     }
-    if (rowloss) rowloss[row] = loss;
+    if (a.none) a.loss[row] = loss;
   }
+  if (t == 0 && a.applied) a.applied[blockIdx.x] = 1.f;
   double d = (double)loss;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o);
   if ((t & 63) == 0) red[t >> 6] = d;
   __syncthreads();
-  if (t == 0) part[blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
+  if (t == 0) a.part[blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-distill_planes_bwd_kernel(const T* __restrict__ z, const int* __restrict__ id,
-                          const float* __restrict__ p, const float4* __restrict__ state,
-                          T* __restrict__ dz, long N, long S, int V, int K, float c, DtScale g) {
-  const long row = blockIdx.x * 256L + threadIdx.x;
-  if (row >= N) return;
+distill_planes_bwd_kernel(const DtArgs a, const DtScale g) {
+  const long row = blockIdx.x * 256L + threadIdx.x, S = a.S;
+  if (a.applied) {  // dz holds the gradient for this upstream already?
+    const float up = *g.up;
+    const bool done = a.applied[blockIdx.x] == up;
+    __syncthreads();
+    if (done) return;
+    if (threadIdx.x == 0) a.applied[blockIdx.x] = up;
+  }
+  if (row >= a.rows) return;
   const long b = row / S, s0 = row - b * S;
-  const T* zr = z + b * V * S + s0;
-  T* dr = dz + b * V * S + s0;
-  const float4 st = state[row];
-  if (st.w == DT_EMPTY) {
-    for (int j = 0; j < V; ++j) st1(dr + (long)j * S, 0.f);
-    return;
-  }
-  const float gs = dt_scale(g, row), cu = st.y * gs;
-  for (int j0 = 0; j0 < V; j0 += 4) {
-    float v[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = j0 + u < V ? ld1(zr + (long)(j0 + u) * S) : 0.f;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (j0 + u < V) st1(dr + (long)(j0 + u) * S, dt_exp2(__builtin_fmaf(v[u], c, -st.x)) * cu);
-  }
-  const long kb = b * K * S + s0;
-  for (int k = 0; k < K; ++k) {
-    const int j = id[kb + k * S];
-    if (j >= 0)
-      st1(dr + (long)j * S, gs * (dt_exp2(__builtin_fmaf(ld1(zr + (long)j * S), c, -st.z)) * st.w -
-                                  p[kb + k * S]));
-  }
+  const T* zr = (const T*)a.z + b * a.V * S + s0;
+  T* dr = (T*)a.dz + b * a.V * S + s0;
+  const long kb = b * a.K * S + s0;
+  const float4 st = a.state[row];
+  if (st.w == DT_EMPTY) dtp_zero(dr, S, a.V);
+  else dtp_gradient(zr, dr, S, a.V, a.K, a.id + kb, a.p + kb, st, a.c, dt_scale(g, row));
 }
 
 // ----------------------------------------------------------------- the loss of all rows
@@ -303,52 +317,153 @@ distill_loss_kernel(const double* __restrict__ part, long n, const int* count, f
   }
 }
 
-extern "C" int accunet_distill_loss(const double* part, long n, const int* count, float* out,
-                                    void* stream) {
-  if (n <= 0) return ACC_EBADSHAPE;
-  if (!part || !out) return ACC_EBADARG;
-  hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, part, n,
-                     count, out);
+// ------------------------------------------------------------------------------- calls
+static long dt_up16(long n) { return (n + 15) / 16 * 16; }
+static bool dt_planes(long S) { return S > 1; }
+// kept for the backward: state, applied, count, id, p
+static long dt_carve_save(DtArgs& a, char* base) {
+  long o = 0;
+  auto take = [&](auto*& ptr, long bytes) {
+    ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(base + o);
+    o = dt_up16(o + bytes);
+  };
+  take(a.state, a.rows * 16);
+  take(a.applied, a.rows * 4);
+  take(a.count, 16);
+  take(a.id, a.rows * a.K * 4);
+  take(a.p, a.rows * a.K * 4);
+  return o;
+}
+static long dt_carve_ws(DtArgs& a, char* base, int dt) {
+  long o = 0;
+  auto take = [&](auto*& ptr, long bytes) {
+    ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(base + o);
+    o = dt_up16(o + bytes);
+  };
+  take(a.tea, a.rows * 8);
+  take(a.part, a.rows * 8);
+  take(a.cnt, a.rows * 4);
+  take(a.ms, dt_planes(a.S) ? 0 : a.rows * dt_rows_runs(a.rows, a.V, dt) * 8);
+  return o;
+}
+static int dt_check(long B, long S, int V, int K, float T) {
+  if (B <= 0 || S <= 0 || B * S > 0x7fffffffL || V <= 0 || V > DT_MAX_V || K <= 0 || K > DT_MAX_K)
+    return ACC_EBADSHAPE;
+  if (dt_planes(S) && V > DTP_MAX_V) return ACC_EBADSHAPE;
+  return T > 0.f && T < INFINITY ? ACC_OK : ACC_EBADARG;
+}
+static DtArgs dt_args(long B, long S, int V, int K, float T, float weight) {
+  DtArgs a = {};
+  a.rows = B * S; a.S = S; a.V = V; a.K = K;
+  a.T = T; a.c = (float)(DT_LOG2E / T); a.weight = weight;
+  a.scale = weight * T * T * DT_LN2;
+  return a;
+}
+
+extern "C" size_t accunet_distill_save_bytes(long B, long S, int V, int K) {
+  if (dt_check(B, S, V, K, 1.f) != ACC_OK) return 0;
+  DtArgs a = dt_args(B, S, V, K, 1.f, 1.f);
+  return (size_t)dt_carve_save(a, nullptr);
+}
+extern "C" size_t accunet_distill_ws_bytes(long B, long S, int V, int K, int dt) {
+  if (dt_check(B, S, V, K, 1.f) != ACC_OK) return 0;
+  DtArgs a = dt_args(B, S, V, K, 1.f, 1.f);
+  return (size_t)dt_carve_ws(a, nullptr, dt);
+}
+// one block a row (or pixel), so the gradient can follow the sum in the same kernel
+extern "C" int accunet_distill_fused(long B, long S, int V, int dt) {
+  return dt_planes(S) || dt_rows_runs(B, V, dt) == 1;
+}
+
+extern "C" int accunet_distill_fwd(const void* z, const void* idx, int idx64, const void* top,
+                                   int top_dt, const float* rest, float* loss, int reduction,
+                                   void* dz, void* save, size_t save_bytes, void* ws,
+                                   size_t ws_bytes, long B, long S, int V, int K, float T,
+                                   float weight, int dt, void* stream) {
+  const int rc = dt_check(B, S, V, K, T);
+  if (rc != ACC_OK) return rc;
+  if (!z || !idx || !top || !loss || !save || !ws || reduction < 0 || reduction > 2 ||
+      (dt != ACC_F32 && dt != ACC_BF16) || (top_dt != ACC_F32 && top_dt != ACC_BF16))
+    return ACC_EBADARG;
+  if (((uintptr_t)save | (uintptr_t)ws) & 15) return ACC_EBADARG;
+  if (dz && (reduction == 0 || !accunet_distill_fused(B, S, V, dt) ||
+             (((uintptr_t)z ^ (uintptr_t)dz) & 15)))
+    return ACC_EBADARG;
+  DtArgs a = dt_args(B, S, V, K, T, weight);
+  if ((size_t)dt_carve_save(a, (char*)save) > save_bytes) return ACC_EBADARG;
+  if ((size_t)dt_carve_ws(a, (char*)ws, dt) > ws_bytes) return ACC_EBADARG;
+  a.z = z; a.rest = rest; a.loss = loss; a.dz = dz;
+  a.none = reduction == 0;
+  a.mean = reduction == 2;
+  if (!dz) a.applied = nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  const bool planes = dt_planes(S);
+  const unsigned pix = (unsigned)((a.rows + 255) / 256), quad = (unsigned)((a.rows + 3) / 4);
+  const int nb = (int)(planes ? pix : quad);
+  // one block counts straight into its place
+  int* cnt = nb == 1 ? a.count : a.cnt;
+  auto teacher = [&](auto itag) {
+    using IT = decltype(itag);
+    with_dt(top_dt, [&](auto tag) {
+      using TT = decltype(tag);
+      if (planes)
+        hipLaunchKernelGGL((distill_teacher_planes_kernel<IT, TT>), dim3(pix), dim3(256), 0, st,
+                           (const IT*)idx, (const TT*)top, rest, a.id, a.p, a.tea, cnt, a.rows, S,
+                           V, K, a.c);
+      else
+        hipLaunchKernelGGL((distill_teacher_rows_kernel<IT, TT>), dim3(quad), dim3(256), 0, st,
+                           (const IT*)idx, (const TT*)top, rest, a.id, a.p, a.tea, cnt, a.rows, V,
+                           K, a.c);
+    });
+  };
+  if (idx64) teacher((long long)0);
+  else teacher((int)0);
+  if (nb > 1 && a.mean)
+    hipLaunchKernelGGL(distill_count_kernel, dim3(1), dim3(1024), 0, st, a.cnt, nb, a.count);
+  if (planes) {
+    const DtScale g = {nullptr, 0, a.mean ? a.count : nullptr, weight * T};
+    with_dt(dt, [&](auto tag) {
+      using Z = decltype(tag);
+      if (rest)
+        hipLaunchKernelGGL((distill_planes_fwd_kernel<Z, true>), dim3(pix), dim3(256),
+                           (V + 31) / 32 * 1024, st, a, g);
+      else
+        hipLaunchKernelGGL((distill_planes_fwd_kernel<Z, false>), dim3(pix), dim3(256), 0, st, a, g);
+    });
+  } else {
+    dt_rows_forward(a, dt, st);
+  }
+  // four rows at most in one block write the loss themselves
+  const bool inside =
+      !planes && nb == 1 && (V <= DTR_WAVE_V || dt_rows_runs(a.rows, V, dt) > 1);
+  if (!a.none && !inside)
+    hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, st, a.part,
+                       planes ? (long)pix : a.rows, a.mean ? a.count : nullptr, loss);
   return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
 }
 
-extern "C" int accunet_distill_planes_fwd(const void* z, const float* rest, const int* id,
-                                          const float* p, const float* tea, float* state,
-                                          float* rowloss, double* part, long B, long S, int V,
-                                          int K, float T, float weight, int dt, void* stream) {
-  if (B <= 0 || S <= 0 || V <= 0 || V > DTP_MAX_V || K <= 0 || K > DT_MAX_K) return ACC_EBADSHAPE;
-  if (!z || !id || !p || !tea || !state || !part || !(T > 0.f)) return ACC_EBADARG;
-  const float c = (float)(DT_LOG2E / T);
-  const float scale = weight * T * T * DT_LN2;
-  const dim3 grid((unsigned)((B * S + 255) / 256));
-  const int rc = with_dt(dt, [&](auto tag) {
-    using Z = decltype(tag);
-    if (rest)
-      hipLaunchKernelGGL((distill_planes_fwd_kernel<Z, true>), grid, dim3(256),
-                         (V + 31) / 32 * 1024, (hipStream_t)stream, (const Z*)z, rest, id, p,
-                         (const float2*)tea, (float4*)state, rowloss, part, B * S, S, V, K, c, scale);
-    else
-      hipLaunchKernelGGL((distill_planes_fwd_kernel<Z, false>), grid, dim3(256), 0,
-                         (hipStream_t)stream, (const Z*)z, rest, id, p, (const float2*)tea,
-                         (float4*)state, rowloss, part, B * S, S, V, K, c, scale);
-  });
+extern "C" int accunet_distill_bwd(const void* z, void* save, size_t save_bytes, const float* up,
+                                   int reduction, int held, void* dz, long B, long S, int V, int K,
+                                   float T, float weight, int dt, void* stream) {
+  const int rc = dt_check(B, S, V, K, T);
   if (rc != ACC_OK) return rc;
-  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
-}
-
-extern "C" int accunet_distill_planes_bwd(const void* z, const int* id, const float* p,
-                                          const float* state, const float* up, int up_rows,
-                                          const int* count, void* dz, long B, long S, int V, int K,
-                                          float T, float weight, int dt, void* stream) {
-  if (B <= 0 || S <= 0 || V <= 0 || V > DTP_MAX_V || K <= 0 || K > DT_MAX_K) return ACC_EBADSHAPE;
-  if (!z || !id || !p || !state || !dz || !(T > 0.f)) return ACC_EBADARG;
-  const DtScale g = {up, up_rows, count, weight * T};
-  const int rc = with_dt(dt, [&](auto tag) {
-    using Z = decltype(tag);
-    hipLaunchKernelGGL(distill_planes_bwd_kernel<Z>, dim3((unsigned)((B * S + 255) / 256)),
-                       dim3(256), 0, (hipStream_t)stream, (const Z*)z, id, p, (const float4*)state,
-                       (Z*)dz, B * S, S, V, K, (float)(DT_LOG2E / T), g);
-  });
-  if (rc != ACC_OK) return rc;
+  if (!z || !save || !up || !dz || reduction < 0 || reduction > 2 || (held && reduction == 0) ||
+      (dt != ACC_F32 && dt != ACC_BF16))
+    return ACC_EBADARG;
+  if ((uintptr_t)save & 15 || (((uintptr_t)z ^ (uintptr_t)dz) & 15)) return ACC_EBADARG;
+  DtArgs a = dt_args(B, S, V, K, T, weight);
+  if ((size_t)dt_carve_save(a, (char*)save) > save_bytes) return ACC_EBADARG;
+  a.z = z; a.dz = dz;
+  if (!held) a.applied = nullptr;
+  const DtScale g = {up, reduction == 0, reduction == 2 ? a.count : nullptr, weight * T};
+  hipStream_t st = (hipStream_t)stream;
+  if (dt_planes(S))
+    with_dt(dt, [&](auto tag) {
+      using Z = decltype(tag);
+      hipLaunchKernelGGL(distill_planes_bwd_kernel<Z>, dim3((unsigned)((a.rows + 255) / 256)),
+                         dim3(256), 0, st, a, g);
+    });
+  else
+    dt_rows_backward(a, g, dt, st);
   return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
 }

@@ -4,13 +4,15 @@
 // its first and last vector may be partial (an odd V puts rows at any address) and are then
 // read and written class by class. Rows up to DTR_WAVE_V classes take one wave each, longer
 // ones blocks of 256 threads, several blocks a row where the rows alone do not fill the
-// card. With a remaining mass the listed classes are kept out of the sum by a byte of marks
+// card. Where one block has a whole row, the gradient for an upstream of 1 is written by the
+// same kernel: the row's second read comes from the caches (rows in flight are kept to about
+// 128 MB by the number of threads a row gets), so the logits cross the memory bus once.
+// With a remaining mass the listed classes are kept out of the sum by a byte of marks
 // per vector in LDS (one read per vector, nearly always zero).
 #include <type_traits>
 
 #include "distill.h"
 
-#define DTR_WAVE_V 2048
 #define DTR_CHUNK 16384  // vectors whose marks are held at once
 
 template <typename T>
@@ -22,7 +24,12 @@ struct DtVec<float> {
     const float4 q = ld4(p);
     v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
   }
-  static ACC_DEV void st(float* p, const float (&v)[4]) { st4(p, make_float4(v[0], v[1], v[2], v[3])); }
+  template <bool STREAM>
+  static ACC_DEV void st(float* p, const float (&v)[4]) {
+    const float4 q = make_float4(v[0], v[1], v[2], v[3]);
+    if (STREAM) st4_nt(p, q);
+    else st4(p, q);
+  }
 };
 template <>
 struct DtVec<bf16_t> {
@@ -32,9 +39,12 @@ struct DtVec<bf16_t> {
     v[0] = bflo(q.x); v[1] = bfhi(q.x); v[2] = bflo(q.y); v[3] = bfhi(q.y);
     v[4] = bflo(q.z); v[5] = bfhi(q.z); v[6] = bflo(q.w); v[7] = bfhi(q.w);
   }
+  template <bool STREAM>
   static ACC_DEV void st(bf16_t* p, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]),
-                                              pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+    const acc_u32x4 q = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]),
+                         pack_bf2(v[6], v[7])};
+    if (STREAM) __builtin_nontemporal_store(q, reinterpret_cast<acc_u32x4*>(p));
+    else *reinterpret_cast<acc_u32x4*>(p) = q;
   }
 };
 
@@ -116,7 +126,7 @@ ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id
 
 // One wave: the row's state and loss from (m, s) over the streamed classes.
 template <typename T>
-ACC_DEV void dt_finish_row(const T* z, const int* id, const float* p, int K, float m, float s,
+ACC_DEV float4 dt_finish_row(const T* z, const int* id, const float* p, int K, float m, float s,
                            float rest, bool has_rest, float h, float c, float scale, int lane,
                            float4* state, float* rowloss, double* part) {
   const float mr = m, sr = s;
@@ -142,8 +152,10 @@ ACC_DEV void dt_finish_row(const T* z, const int* id, const float* p, int K, flo
     if (rowloss) *rowloss = loss;
     *part = (double)loss;
   }
+  return o.state;
 }
 
+// One wave: a row that does not count.
 ACC_DEV void dt_empty_row(int lane, float4* state, float* rowloss, double* part) {
   if (lane == 0) {
     *state = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
@@ -152,137 +164,217 @@ ACC_DEV void dt_empty_row(int lane, float4* state, float* rowloss, double* part)
   }
 }
 
-// short rows: one wave a row, everything in one pass
-template <typename T, bool REST>
-__global__ void __launch_bounds__(256)
-distill_rows_wave_kernel(const T* __restrict__ z, const float* __restrict__ rest,
-                         const int* __restrict__ id, const float* __restrict__ p,
-                         const float2* __restrict__ tea, float4* __restrict__ state,
-                         float* __restrict__ rowloss, double* __restrict__ part, long R, int V,
-                         int K, float c, float scale) {
-  __shared__ unsigned mark[4][(DTR_WAVE_V / 4 + 2 + 3) / 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long row = blockIdx.x * 4L + wave;
-  if (row >= R) return;
-  float* rl = rowloss ? rowloss + row : nullptr;
-  const float2 te = tea[row];
-  if (te.y == 0.f) {
-    dt_empty_row(lane, state + row, rl, part + row);
-    return;
-  }
-  const T* zr = z + row * V;
-  const int off = dt_offset(zr);
-  float m = -INFINITY, s = 0.f;
-  dt_stream<T, REST, 64>(zr, off, V, 0, (off + V + DtVec<T>::N - 1) / DtVec<T>::N, id + row * K, K,
-                         lane, mark[wave], c, m, s);
-  dt_wave_join(m, s, c);
-  dt_finish_row(zr, id + row * K, p + row * K, K, m, s, REST ? rest[row] : 0.f, REST, te.x, c,
-                scale, lane, state + row, rl, part + row);
-}
-
-// long rows: block (x, row) streams the x-th run of vectors into ms[row][x]
-template <typename T, bool REST>
-__global__ void __launch_bounds__(256)
-distill_rows_sum_kernel(const T* __restrict__ z, const int* __restrict__ id,
-                        const float2* __restrict__ tea, float2* __restrict__ ms, int V, int K,
-                        int run, float c) {
-  __shared__ unsigned mark[REST ? DTR_CHUNK / 4 : 1];
-  __shared__ float2 red[4];
-  const long r = blockIdx.x;
-  if (tea[r].y == 0.f) return;
-  const T* zr = z + r * V;
-  const int off = dt_offset(zr);
-  const int nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
-  const int q0 = min(nq, (int)blockIdx.y * run), q1 = min(nq, q0 + run);
-  float m = -INFINITY, s = 0.f;
-  dt_stream<T, REST, 256>(zr, off, V, q0, q1, id + r * K, K, threadIdx.x, mark, c, m, s);
-  dt_wave_join(m, s, c);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(m, s);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 4; ++w) dt_join(m, s, red[w].x, red[w].y, c);
-    ms[r * gridDim.y + blockIdx.y] = make_float2(m, s);
-  }
-}
-
-template <typename T, bool REST>
-__global__ void __launch_bounds__(256)
-distill_rows_finish_kernel(const T* __restrict__ z, const float* __restrict__ rest,
-                           const int* __restrict__ id, const float* __restrict__ p,
-                           const float2* __restrict__ tea, const float2* __restrict__ ms, int runs,
-                           float4* __restrict__ state, float* __restrict__ rowloss,
-                           double* __restrict__ part, long R, int V, int K, float c, float scale) {
-  const int lane = threadIdx.x & 63;
-  const long row = blockIdx.x * 4L + (threadIdx.x >> 6);
-  if (row >= R) return;
-  float* rl = rowloss ? rowloss + row : nullptr;
-  const float2 te = tea[row];
-  if (te.y == 0.f) {
-    dt_empty_row(lane, state + row, rl, part + row);
-    return;
-  }
-  float m = -INFINITY, s = 0.f;
-  for (int i = lane; i < runs; i += 64) {
-    const float2 v = ms[row * runs + i];
-    dt_join(m, s, v.x, v.y, c);
-  }
-  dt_wave_join(m, s, c);
-  dt_finish_row(z + row * V, id + row * K, p + row * K, K, m, s, REST ? rest[row] : 0.f, REST,
-                te.x, c, scale, lane, state + row, rl, part + row);
-}
-
-// Gradient: every class as not listed, then, behind a barrier (the block's own stores),
-// the listed classes of this run over it. NT threads a row, run vectors each.
-template <typename T, int NT>
-__global__ void __launch_bounds__(256)
-distill_rows_bwd_kernel(const T* __restrict__ z, const int* __restrict__ id,
-                        const float* __restrict__ p, const float4* __restrict__ state,
-                        T* __restrict__ dz, long R, int V, int K, int run, float c, DtScale g) {
+// Gradient of vectors [q0, q1) of a row by threads t of NT: every class as not listed, then,
+// behind a barrier, the listed classes over it. `dr` has z's alignment (checked by the host).
+// STREAM: stored past the caches.
+template <typename T, int NT, bool STREAM>
+ACC_DEV void dt_gradient(const T* zr, T* dr, int off, int V, int q0, int q1, const int* id,
+                         const float* p, int K, int t, const float4& st, float c, float gs) {
   constexpr int N = DtVec<T>::N;
-  const int t = NT == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  const long row = NT == 64 ? blockIdx.x * 4L + (threadIdx.x >> 6) : (long)blockIdx.x;
-  if (NT == 64 && row >= R) return;
-  const T* zr = z + row * V;
-  T* dr = dz + row * V;
-  const int off = dt_offset(zr);  // dz has z's alignment (checked by the host)
-  const int nq = (off + V + N - 1) / N;
-  const int q0 = min(nq, (int)blockIdx.y * run), q1 = min(nq, q0 + run);
-  const float4 st = state[row];
+  constexpr int U = 4;
   const bool live = !(st.w == DT_EMPTY);
-  const float gs = live ? dt_scale(g, row) : 0.f, cu = live ? st.y * gs : 0.f;
-  for (int q = q0 + t; q < q1; q += NT) {
-    float v[N];
+  const float cu = st.y * gs;
+  for (int q = q0 + t; q < q1; q += NT * U) {
+    float v[U][N];
     if (live) {
-      dt_load(zr, off, V, q, v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = dt_exp2(__builtin_fmaf(v[e], c, -st.x)) * cu;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = 0.f;
+      for (int u = 0; u < U; ++u)
+        if (q + u * NT < q1) dt_load(zr, off, V, q + u * NT, v[u]);
     }
-    const int j = q * N - off;
-    if (j >= 0 && j + N <= V) {
-      DtVec<T>::st(dr + j, v);
-    } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (q + u * NT >= q1) continue;
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (j + e >= 0 && j + e < V) st1(dr + j + e, v[e]);
+        v[u][e] = live ? dt_exp2(__builtin_fmaf(v[u][e], c, -st.x)) * cu : 0.f;
+      const int j = (q + u * NT) * N - off;
+      if (j >= 0 && j + N <= V) {
+        DtVec<T>::template st<STREAM>(dr + j, v[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (j + e >= 0 && j + e < V) st1(dr + j + e, v[u][e]);
+      }
     }
   }
-  if (!live) return;
+  if (!live) return;  // the same for the whole row
   __threadfence_block();
   if (NT > 64) __syncthreads();
   else __builtin_amdgcn_s_waitcnt(0);  // one wave: its stores are done before the next ones
   for (int k = t; k < K; k += NT) {
-    const int j = id[row * K + k];
+    const int j = id[k];
     const int q = (j + off) / N;
     if (j >= 0 && q >= q0 && q < q1)
-      st1(dr + j, gs * (dt_exp2(__builtin_fmaf(ld1(zr + j), c, -st.z)) * st.w - p[row * K + k]));
+      st1(dr + j, gs * (dt_exp2(__builtin_fmaf(ld1(zr + j), c, -st.z)) * st.w - p[k]));
   }
 }
 
-// runs of vectors a long row is cut into: enough blocks for the card, 1024 vectors at least
-static int dt_runs(long R, int V, int dt) {
+// four rows at most (one block): their loss without another kernel
+ACC_DEV void dt_small_loss(const DtArgs& a, double* red) {
+  if (gridDim.x != 1 || a.none) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int w = 0; w < 4; ++w) t += w < a.rows ? red[w] : 0.0;
+    if (a.mean) t /= (double)max(*a.count, 1);
+    a.loss[0] = (float)t;
+  }
+}
+
+// short rows: one wave a row, everything in one pass
+template <typename T, bool REST>
+__global__ void __launch_bounds__(256)
+distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
+  __shared__ unsigned mark[4][(DTR_WAVE_V / 4 + 2 + 3) / 4];
+  __shared__ double red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row = blockIdx.x * 4L + wave;
+  const int V = a.V, K = a.K;
+  if (row < a.rows) {
+    float* rl = a.none ? a.loss + row : nullptr;
+    const float2 te = a.tea[row];
+    const T* zr = (const T*)a.z + row * V;
+    const int off = dt_offset(zr), nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
+    float4 st = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
+    if (te.y == 0.f) {
+      dt_empty_row(lane, a.state + row, rl, &red[wave]);
+    } else {
+      float m = -INFINITY, s = 0.f;
+      dt_stream<T, REST, 64>(zr, off, V, 0, nq, a.id + row * K, K, lane, mark[wave], a.c, m, s);
+      dt_wave_join(m, s, a.c);
+      st = dt_finish_row(zr, a.id + row * K, a.p + row * K, K, m, s, REST ? a.rest[row] : 0.f, REST,
+                         te.x, a.c, a.scale, lane, a.state + row, rl, &red[wave]);
+    }
+    if (lane == 0) {
+      a.part[row] = red[wave];
+      if (a.applied) a.applied[row] = 1.f;
+    }
+    if (a.dz)
+      dt_gradient<T, 64, false>(zr, (T*)a.dz + row * V, off, V, 0, nq, a.id + row * K,
+                                a.p + row * K, K, lane, st, a.c, dt_scale(g, row));
+  }
+  dt_small_loss(a, red);
+}
+
+// long rows, one block each: the sum, the row's loss and the gradient
+template <typename T, bool REST, int NT, bool STREAM>
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8)))
+distill_rows_fused_kernel(const DtArgs a, const DtScale g) {
+  __shared__ unsigned mark[REST ? DTR_CHUNK / 4 : 1];
+  __shared__ float2 red[NT / 64];
+  __shared__ float4 rs;
+  const long row = blockIdx.x;
+  const int t = threadIdx.x, V = a.V, K = a.K;
+  const T* zr = (const T*)a.z + row * V;
+  const int off = dt_offset(zr), nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
+  float* rl = a.none ? a.loss + row : nullptr;
+  const float2 te = a.tea[row];
+  float4 st = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
+  if (te.y == 0.f) {
+    dt_empty_row(t, a.state + row, rl, a.part + row);
+  } else {
+    float m = -INFINITY, s = 0.f;
+    dt_stream<T, REST, NT>(zr, off, V, 0, nq, a.id + row * K, K, t, mark, a.c, m, s);
+    dt_wave_join(m, s, a.c);
+    if ((t & 63) == 0) red[t >> 6] = make_float2(m, s);
+    __syncthreads();
+    if (t < 64) {
+      m = red[0].x;
+      s = red[0].y;
+      for (int w = 1; w < NT / 64; ++w) dt_join(m, s, red[w].x, red[w].y, a.c);
+      st = dt_finish_row(zr, a.id + row * K, a.p + row * K, K, m, s, REST ? a.rest[row] : 0.f, REST,
+                         te.x, a.c, a.scale, t, a.state + row, rl, a.part + row);
+      if (t == 0) rs = st;
+    }
+    __syncthreads();
+    st = rs;
+  }
+  if (t == 0 && a.applied) a.applied[row] = 1.f;
+  if (a.dz)
+    dt_gradient<T, NT, STREAM>(zr, (T*)a.dz + row * V, off, V, 0, nq, a.id + row * K, a.p + row * K,
+                               K, t, st, a.c, dt_scale(g, row));
+}
+
+// long rows, several blocks each: block (row, y) streams the y-th run into ms[row][y]
+template <typename T, bool REST>
+__global__ void __launch_bounds__(256)
+distill_rows_sum_kernel(const DtArgs a, int run) {
+  __shared__ unsigned mark[REST ? DTR_CHUNK / 4 : 1];
+  __shared__ float2 red[4];
+  const long r = blockIdx.x;
+  const int V = a.V, K = a.K;
+  if (a.tea[r].y == 0.f) return;
+  const T* zr = (const T*)a.z + r * V;
+  const int off = dt_offset(zr);
+  const int nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
+  const int q0 = min(nq, (int)blockIdx.y * run), q1 = min(nq, q0 + run);
+  float m = -INFINITY, s = 0.f;
+  dt_stream<T, REST, 256>(zr, off, V, q0, q1, a.id + r * K, K, threadIdx.x, mark, a.c, m, s);
+  dt_wave_join(m, s, a.c);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) dt_join(m, s, red[w].x, red[w].y, a.c);
+    a.ms[r * gridDim.y + blockIdx.y] = make_float2(m, s);
+  }
+}
+
+template <typename T, bool REST>
+__global__ void __launch_bounds__(256)
+distill_rows_finish_kernel(const DtArgs a, int runs) {
+  __shared__ double red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row = blockIdx.x * 4L + wave;
+  const int V = a.V, K = a.K;
+  if (row < a.rows) {
+    float* rl = a.none ? a.loss + row : nullptr;
+    const float2 te = a.tea[row];
+    if (te.y == 0.f) {
+      dt_empty_row(lane, a.state + row, rl, &red[wave]);
+    } else {
+      float m = -INFINITY, s = 0.f;
+      for (int i = lane; i < runs; i += 64) {
+        const float2 v = a.ms[row * runs + i];
+        dt_join(m, s, v.x, v.y, a.c);
+      }
+      dt_wave_join(m, s, a.c);
+      dt_finish_row((const T*)a.z + row * V, a.id + row * K, a.p + row * K, K, m, s,
+                    REST ? a.rest[row] : 0.f, REST, te.x, a.c, a.scale, lane, a.state + row, rl,
+                    &red[wave]);
+    }
+    if (lane == 0) a.part[row] = red[wave];
+  }
+  dt_small_loss(a, red);
+}
+
+// The gradient from the kept state. NT threads a row (or a run of it).
+template <typename T, int NT, bool STREAM>
+__global__ void __launch_bounds__(256)
+distill_rows_bwd_kernel(const DtArgs a, const DtScale g, int run) {
+  const int t = NT == 64 ? (threadIdx.x & 63) : threadIdx.x;
+  const long row = NT == 64 ? blockIdx.x * 4L + (threadIdx.x >> 6) : (long)blockIdx.x;
+  if (NT == 64 && row >= a.rows) return;
+  if (a.applied) {  // dz holds the gradient for this upstream already? (one run a row)
+    const float up = *g.up;
+    const bool done = a.applied[row] == up;
+    if (NT > 64) __syncthreads();
+    if (done) return;
+    if (t == 0) a.applied[row] = up;
+  }
+  const int V = a.V, K = a.K;
+  const T* zr = (const T*)a.z + row * V;
+  const int off = dt_offset(zr);
+  const int nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
+  const int q0 = min(nq, (int)blockIdx.y * run), q1 = min(nq, q0 + run);
+  const float4 st = a.state[row];
+  dt_gradient<T, NT, STREAM>(zr, (T*)a.dz + row * V, off, V, q0, q1, a.id + row * K, a.p + row * K,
+                             K, t, st, a.c, st.w == DT_EMPTY ? 0.f : dt_scale(g, row));
+}
+
+// runs of vectors a long row is cut into: one where the rows alone give every CU a block,
+// else enough for 8 blocks a CU, 1024 vectors at least
+int dt_rows_runs(long R, int V, int dt) {
+  if (V <= DTR_WAVE_V || R >= 256) return 1;
   const int n = dt == ACC_F32 ? 4 : 8;
   const long nq = ((long)V + n - 1) / n + 1;
   const long want = (2048 + R - 1) / R, most = (nq + 1023) / 1024;
@@ -292,71 +384,61 @@ static int dt_run_len(int runs, int V, int dt) {
   const int n = dt == ACC_F32 ? 4 : 8;
   return ceil_div(((long)V + n - 1) / n + 1, runs);
 }
+// gradients of 64 MB and more are streamed (the last-level cache holds 256 MB)
+template <typename T>
+static bool dt_large(const DtArgs& a) { return a.rows * a.V * (long)sizeof(T) >= (64L << 20); }
 
-extern "C" size_t accunet_distill_rows_ws_elems(long R, int V, int dt) {
-  if (R <= 0 || V <= 0 || V <= DTR_WAVE_V) return 0;
-  return (size_t)R * dt_runs(R, V, dt) * 2;
-}
-
-extern "C" int accunet_distill_rows_fwd(const void* z, const float* rest, const int* id,
-                                        const float* p, const float* tea, float* state,
-                                        float* rowloss, double* part, float* ws, size_t ws_elems,
-                                        long R, int V, int K, float T, float weight, int dt,
-                                        void* stream) {
-  if (R <= 0 || R > 0x7fffffffL || V <= 0 || V > DT_MAX_V || K <= 0 || K > DT_MAX_K) return ACC_EBADSHAPE;
-  if (!z || !id || !p || !tea || !state || !part || !(T > 0.f)) return ACC_EBADARG;
-  if (ws_elems < accunet_distill_rows_ws_elems(R, V, dt)) return ACC_EBADARG;
-  const float c = (float)(DT_LOG2E / T);
-  const float scale = weight * T * T * DT_LN2;
-  hipStream_t st = (hipStream_t)stream;
-  const int rc = with_dt(dt, [&](auto tag) {
+void dt_rows_forward(const DtArgs& a, int dt, hipStream_t st) {
+  const DtScale g = {nullptr, 0, a.mean ? a.count : nullptr, a.weight * a.T};
+  with_dt(dt, [&](auto tag) {
     using Z = decltype(tag);
     auto go = [&](auto rtag) {
       constexpr bool REST = decltype(rtag)::value;
-      const dim3 g4((unsigned)((R + 3) / 4));
-      if (V <= DTR_WAVE_V) {
-        hipLaunchKernelGGL((distill_rows_wave_kernel<Z, REST>), g4, dim3(256), 0, st, (const Z*)z,
-                           rest, id, p, (const float2*)tea, (float4*)state, rowloss, part, R, V, K,
-                           c, scale);
+      const dim3 g4((unsigned)((a.rows + 3) / 4));
+      if (a.V <= DTR_WAVE_V) {
+        hipLaunchKernelGGL((distill_rows_wave_kernel<Z, REST>), g4, dim3(256), 0, st, a, g);
         return;
       }
-      const int runs = dt_runs(R, V, dt);
-      hipLaunchKernelGGL((distill_rows_sum_kernel<Z, REST>), dim3((unsigned)R, runs), dim3(256), 0,
-                         st, (const Z*)z, id, (const float2*)tea, (float2*)ws, V, K,
-                         dt_run_len(runs, V, dt), c);
-      hipLaunchKernelGGL((distill_rows_finish_kernel<Z, REST>), g4, dim3(256), 0, st, (const Z*)z,
-                         rest, id, p, (const float2*)tea, (const float2*)ws, runs, (float4*)state,
-                         rowloss, part, R, V, K, c, scale);
+      const int runs = dt_rows_runs(a.rows, a.V, dt);
+      if (runs == 1) {
+        // threads a row: a CU's 2048 hold at most 512 KB of rows
+        const long bytes = (long)a.V * sizeof(Z);
+        const dim3 grid((unsigned)a.rows);
+        auto nt = [&](auto ntag) {
+          constexpr int NT = decltype(ntag)::value;
+          if (dt_large<Z>(a))
+            hipLaunchKernelGGL((distill_rows_fused_kernel<Z, REST, NT, true>), grid, dim3(NT), 0,
+                               st, a, g);
+          else
+            hipLaunchKernelGGL((distill_rows_fused_kernel<Z, REST, NT, false>), grid, dim3(NT), 0,
+                               st, a, g);
+        };
+        if (bytes <= (64 << 10)) nt(std::integral_constant<int, 256>{});
+        else if (bytes <= (128 << 10)) nt(std::integral_constant<int, 512>{});
+        else nt(std::integral_constant<int, 1024>{});
+        return;
+      }
+      hipLaunchKernelGGL((distill_rows_sum_kernel<Z, REST>), dim3((unsigned)a.rows, runs),
+                         dim3(256), 0, st, a, dt_run_len(runs, a.V, dt));
+      hipLaunchKernelGGL((distill_rows_finish_kernel<Z, REST>), g4, dim3(256), 0, st, a, runs);
     };
-    if (rest) go(std::true_type{});
+    if (a.rest) go(std::true_type{});
     else go(std::false_type{});
   });
-  if (rc != ACC_OK) return rc;
-  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
 }
 
-extern "C" int accunet_distill_rows_bwd(const void* z, const int* id, const float* p,
-                                        const float* state, const float* up, int up_rows,
-                                        const int* count, void* dz, long R, int V, int K, float T,
-                                        float weight, int dt, void* stream) {
-  if (R <= 0 || R > 0x7fffffffL || V <= 0 || V > DT_MAX_V || K <= 0 || K > DT_MAX_K) return ACC_EBADSHAPE;
-  if (!z || !id || !p || !state || !dz || !(T > 0.f)) return ACC_EBADARG;
-  if (((uintptr_t)z ^ (uintptr_t)dz) & 15) return ACC_EBADARG;
-  const float c = (float)(DT_LOG2E / T);
-  const DtScale g = {up, up_rows, count, weight * T};
-  const int rc = with_dt(dt, [&](auto tag) {
+void dt_rows_backward(const DtArgs& a, const DtScale& g, int dt, hipStream_t st) {
+  with_dt(dt, [&](auto tag) {
     using Z = decltype(tag);
-    if (V <= DTR_WAVE_V) {
-      hipLaunchKernelGGL((distill_rows_bwd_kernel<Z, 64>), dim3((unsigned)((R + 3) / 4)), dim3(256),
-                         0, (hipStream_t)stream, (const Z*)z, id, p, (const float4*)state, (Z*)dz,
-                         R, V, K, dt_run_len(1, V, dt), c, g);
-    } else {
-      const int runs = dt_runs(R, V, dt);
-      hipLaunchKernelGGL((distill_rows_bwd_kernel<Z, 256>), dim3((unsigned)R, runs), dim3(256), 0,
-                         (hipStream_t)stream, (const Z*)z, id, p, (const float4*)state, (Z*)dz, R,
-                         V, K, dt_run_len(runs, V, dt), c, g);
-    }
+    const int runs = dt_rows_runs(a.rows, a.V, dt), len = dt_run_len(runs, a.V, dt);
+    if (a.V <= DTR_WAVE_V)
+      hipLaunchKernelGGL((distill_rows_bwd_kernel<Z, 64, false>),
+                         dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a, g, len);
+    else if (dt_large<Z>(a))
+      hipLaunchKernelGGL((distill_rows_bwd_kernel<Z, 256, true>), dim3((unsigned)a.rows, runs),
+                         dim3(256), 0, st, a, g, len);
+    else
+      hipLaunchKernelGGL((distill_rows_bwd_kernel<Z, 256, false>), dim3((unsigned)a.rows, runs),
+                         dim3(256), 0, st, a, g, len);
   });
-  if (rc != ACC_OK) return rc;
-  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
 }

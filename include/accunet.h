@@ -522,35 +522,25 @@ int accunet_blocknorm_bwd(const void* x, const void* f, const float* w1, const f
  *   p = (1 - rest) softmax(top / T), q = softmax(z / T)
  *   loss = weight T^2 [sum p (log p - log q) + rest (log rest - log q(not listed))]
  * A row without a valid entry has loss 0 and gradient 0.
- *   accunet_distill_teacher: id [.][K] int32 (each class once, -1 elsewhere), p [.][K] fp32,
- *     tea [rows][2] fp32, *count (int32, zeroed by the caller) += rows with an entry. S = 1
- *     for "rows" (B = R).
- *   accunet_distill_rows_fwd / _planes_fwd: state [rows][4] fp32, rowloss [rows] fp32 (or
- *     NULL), part fp64 (rows: [R], planes: [ceil(B*S/256)]); ws: fp32 scratch of
- *     accunet_distill_rows_ws_elems elements.
- *   accunet_distill_loss: out = sum of the n values of part, / *count where count is given.
- *   accunet_distill_rows_bwd / _planes_bwd: dz (z's type, shape and address modulo 16),
- *     scaled by the upstream gradient up (one value, or one a row with up_rows; NULL: 1) and
- *     1 / *count where count is given.
+ *   accunet_distill_fwd: loss (one value; one a row with reduction 0). reduction: 0 none, 1
+ *     sum, 2 mean over the rows with an entry. S = 1 for "rows" (B = R). save (kept for the
+ *     backward) and ws (scratch): accunet_distill_save_bytes / _ws_bytes bytes, 16-byte
+ *     aligned. dz (or NULL; reduction 1, 2 and accunet_distill_fused only): the gradient for
+ *     an upstream gradient of 1 in the same pass.
+ *   accunet_distill_bwd: dz (z's type, shape and address modulo 16) scaled by the upstream
+ *     gradient `up` (one value, one a row with reduction 0). held != 0: dz is the tensor that
+ *     the forward filled; it is rewritten only where `up` is not what it holds.
  * ------------------------------------------------------------------------- */
-int accunet_distill_teacher(const void* idx, int idx64, const void* top, int top_dt,
-                            const float* rest, int* id, float* p, float* tea, int* count, long B,
-                            long S, int V, int K, float T, void* stream);
-size_t accunet_distill_rows_ws_elems(long R, int V, int dt);
-int accunet_distill_rows_fwd(const void* z, const float* rest, const int* id, const float* p,
-                             const float* tea, float* state, float* rowloss, double* part,
-                             float* ws, size_t ws_elems, long R, int V, int K, float T,
-                             float weight, int dt, void* stream);
-int accunet_distill_rows_bwd(const void* z, const int* id, const float* p, const float* state,
-                             const float* up, int up_rows, const int* count, void* dz, long R,
-                             int V, int K, float T, float weight, int dt, void* stream);
-int accunet_distill_planes_fwd(const void* z, const float* rest, const int* id, const float* p,
-                               const float* tea, float* state, float* rowloss, double* part, long B,
-                               long S, int V, int K, float T, float weight, int dt, void* stream);
-int accunet_distill_planes_bwd(const void* z, const int* id, const float* p, const float* state,
-                               const float* up, int up_rows, const int* count, void* dz, long B,
-                               long S, int V, int K, float T, float weight, int dt, void* stream);
-int accunet_distill_loss(const double* part, long n, const int* count, float* out, void* stream);
+size_t accunet_distill_save_bytes(long B, long S, int V, int K);
+size_t accunet_distill_ws_bytes(long B, long S, int V, int K, int dt);
+int accunet_distill_fused(long B, long S, int V, int dt);
+int accunet_distill_fwd(const void* z, const void* idx, int idx64, const void* top, int top_dt,
+                        const float* rest, float* loss, int reduction, void* dz, void* save,
+                        size_t save_bytes, void* ws, size_t ws_bytes, long B, long S, int V, int K,
+                        float T, float weight, int dt, void* stream);
+int accunet_distill_bwd(const void* z, void* save, size_t save_bytes, const float* up,
+                        int reduction, int held, void* dz, long B, long S, int V, int K, float T,
+                        float weight, int dt, void* stream);
 
 /* ------------------------------------------------------------------------- *
  * 8-bit linear layer: e4m3 values with a power-of-two scale for each block of 128 along the

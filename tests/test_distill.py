@@ -36,20 +36,25 @@ def test_refusals_on_the_host():
             f(z, i, t, temperature=bad)
     lib = _lib.load()
     ok = 16
-    tea = lib.accunet_distill_teacher
-    assert tea(ok, 1, ok, 0, None, ok, ok, ok, ok, 2, 1, 5, 257, 1.0, None) == -1
-    assert tea(ok, 1, ok, 0, None, ok, ok, ok, ok, 0, 1, 5, 3, 1.0, None) == -1
-    assert tea(ok, 1, ok, 2, None, ok, ok, ok, ok, 2, 1, 5, 3, 1.0, None) == -2
-    assert tea(ok, 1, ok, 0, None, ok, ok, ok, ok, 2, 1, 5, 3, 0.0, None) == -2
-    fwd = lib.accunet_distill_rows_fwd
-    n = lib.accunet_distill_rows_ws_elems(3, 50021, 0)
-    assert n > 0 and lib.accunet_distill_rows_ws_elems(3, 100, 0) == 0
-    assert fwd(ok, None, ok, ok, ok, ok, None, ok, ok, n - 1, 3, 50021, 4, 1.0, 1.0, 0, None) == -2
-    bwd = lib.accunet_distill_rows_bwd
-    assert bwd(16, ok, ok, ok, None, 0, None, 24, 3, 100, 4, 1.0, 1.0, 0, None) == -2  # addresses
-    assert lib.accunet_distill_planes_fwd(ok, None, ok, ok, ok, ok, None, ok, 2, 9, 1025, 4, 1.0,
-                                          1.0, 0, None) == -1
-    assert lib.accunet_distill_loss(ok, 0, None, ok, None) == -1
+    fwd, bwd = lib.accunet_distill_fwd, lib.accunet_distill_bwd
+
+    def f_(R=2, S=1, V=5, K=3, T=1.0, dt=0, red=2, dz=None, z=ok, top_dt=0, short=0, save=16):
+        n, m = lib.accunet_distill_save_bytes(2, 1, 5, 3), lib.accunet_distill_ws_bytes(2, 1, 5, 3, 0)
+        return fwd(z, ok, 1, ok, top_dt, None, ok, red, dz, save, n - short, ok, m, R, S, V, K, T,
+                   1.0, dt, None)
+
+    assert f_(K=257) == -1 and f_(R=0) == -1 and f_(S=9, V=1025) == -1 and f_(V=0) == -1
+    assert f_(top_dt=2) == -2 and f_(dt=2) == -2 and f_(T=0.0) == -2 and f_(red=3) == -2
+    assert f_(z=None) == -2 and f_(short=1) == -2 and f_(save=8) == -2
+    assert f_(dz=24) == -2 and f_(dz=16, red=0) == -2   # dz at another address modulo 16; no sum
+    n = lib.accunet_distill_save_bytes(3, 1, 100, 4)
+    assert bwd(16, ok, n, ok, 2, 0, 24, 3, 1, 100, 4, 1.0, 1.0, 0, None) == -2  # addresses
+    assert bwd(16, ok, n - 1, ok, 2, 0, 16, 3, 1, 100, 4, 1.0, 1.0, 0, None) == -2
+    assert bwd(16, ok, n, ok, 0, 1, 16, 3, 1, 100, 4, 1.0, 1.0, 0, None) == -2  # held, no sum
+    # a few long rows are cut over blocks: no gradient in the forward
+    assert lib.accunet_distill_fused(3, 1, 50021, 0) == 0
+    assert lib.accunet_distill_fused(300, 1, 50021, 0) == 1
+    assert lib.accunet_distill_fused(3, 1, 2048, 0) == 1 and lib.accunet_distill_fused(2, 9, 5, 0) == 1
 
 
 # ----------------------------------------------------------------------- the reference
@@ -300,6 +305,102 @@ def test_gradient_against_differences():
     want = (value(h) - value(-h)) / (2 * h)
     have = float((g.double().cpu() * v).sum())
     assert abs(have - want) <= 1e-6 * float((g.double().cpu() * v).abs().sum()) + 1e-7
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V,K", [(260, 2049, 9), (300, 33001, 5), (257, 70001, 64), (1030, 21, 3)])
+def test_many_rows(R, V, K, dtype):
+    """One block a row, each number of threads; the loss checked on every row, the gradient
+    on rows spread over the batch (the 64-bit reference is a loop)."""
+    z, idx, top, r = _make(R, V, 1, dtype, True)
+    g = torch.Generator().manual_seed(5)
+    idx = torch.randint(0, V, (R, K), generator=g)
+    top = torch.randn(R, K, generator=g).to(dtype)
+    idx[R // 2] = -1
+    pick = [0, 1, R // 2, R - 2, R - 1]
+    loss64, dz64, tl, td, live = _reference(z[pick], idx[pick], top[pick], r[pick], 1.7)
+    zd = z.cuda().requires_grad_()
+    args = (idx.cuda(), top.cuda())
+    kw = dict(rest=r.cuda(), temperature=1.7)
+    per = _fn()(zd, *args, reduction="none", **kw)
+    _close(per[pick], loss64, tl, "loss")
+    (dn,) = torch.autograd.grad(per, zd, torch.ones_like(per))
+    _close(dn[pick], dz64, td, "dz none")
+    n = R - 1
+    mean = _fn()(zd, *args, **kw)
+    want = per.detach().double().sum() / n
+    assert abs(float(mean) - float(want)) <= 4 * U * abs(float(want))
+    (dm,) = torch.autograd.grad(mean, zd)
+    _close(dm[pick], dz64 / n, (td + 8 * U * dz64.abs()) / n, "dz mean")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["rows", "long", "planes"])
+def test_held_gradient(layout):
+    """The forward's gradient is handed out once; other upstream gradients, a second backward
+    of the same graph and an accumulated leaf are right too."""
+    f = _fn()
+    R, V = {"rows": (24, 500), "long": (260, 5001), "planes": (24, 21)}[layout]
+    z, idx, top, r = (t.cuda() for t in _make(R, V, 6, torch.float32, True))
+    dim = -1
+    if layout == "planes":
+        z, idx, top = (t.view(2, R // 2, -1).movedim(-1, 1).contiguous() for t in (z, idx, top))
+        r, dim = r.view(2, R // 2), 1
+
+    def grad(up, **kw):
+        zz = z.clone().requires_grad_()
+        loss = f(zz, idx, top, rest=r, dim=dim, **kw)
+        return torch.autograd.grad(loss, zz, torch.full_like(loss, up))[0]
+
+    one = grad(1.0)
+    for up in (0.5, -2.0, 4.0):  # powers of two: exact
+        assert torch.equal(grad(up), one * up)
+        assert torch.equal(grad(1.0, weight=up), one * up)
+    assert torch.equal(grad(0.0), torch.zeros_like(one))
+    zz = z.clone().requires_grad_()
+    loss = f(zz, idx, top, rest=r, dim=dim)
+    a = torch.autograd.grad(loss, zz, retain_graph=True)[0]
+    b = torch.autograd.grad(loss, zz, torch.full_like(loss, 2.0), retain_graph=True)[0]
+    c = torch.autograd.grad(loss, zz)[0]
+    assert torch.equal(a, one) and torch.equal(b, 2 * one) and torch.equal(c, one)
+    assert len({a.data_ptr(), b.data_ptr(), c.data_ptr()}) == 3
+    zz = z.clone().requires_grad_()
+    f(zz, idx, top, rest=r, dim=dim).backward()
+    f(zz, idx, top, rest=r, dim=dim).backward()
+    assert torch.equal(zz.grad, one + one)
+    with torch.no_grad():
+        v = f(z, idx, top, rest=r, dim=dim)
+    assert torch.equal(v, loss.detach())
+
+
+@pytest.mark.gpu
+def test_backward_alone_captured():
+    """The forward runs eagerly, its backward is captured and replayed with other upstream
+    gradients: each replay writes what its upstream asks for."""
+    f = _fn()
+    z, idx, top, r = (t.cuda() for t in _make(24, 500, 6, torch.float32, True))
+    want = {}
+    for up in (1.0, 0.5, 2.0):
+        zz = z.clone().requires_grad_()
+        loss = f(zz, idx, top, rest=r)
+        want[up] = torch.autograd.grad(loss, zz, torch.full_like(loss, up))[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        zz = z.clone().requires_grad_()
+        loss = f(zz, idx, top, rest=r)
+        up = torch.ones_like(loss)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            (dz,) = torch.autograd.grad(loss, zz, up)
+    for u in (2.0, 1.0, 1.0, 0.5, 1.0):
+        up.fill_(u)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dz, want[u]), u
 
 
 @pytest.mark.gpu
