@@ -127,7 +127,8 @@ struct DtArgs {
 };
 
 // rows with the classes last (distill_rows.hip); up to DTR_WAVE_V classes a wave has a row
-#define DTR_WAVE_V 2048
+// in registers (512 vectors of 4 fp32 at most, partial ones at both ends included)
+#define DTR_WAVE_V 2032
 int dt_rows_runs(long R, int V, int dt);
 void dt_rows_forward(const DtArgs& a, int dt, hipStream_t st);
 void dt_rows_backward(const DtArgs& a, const DtScale& g, int dt, hipStream_t st);

@@ -385,7 +385,7 @@ extern "C" int accunet_distill_fwd(const void* z, const void* idx, int idx64, co
   if (!z || !idx || !top || !loss || !save || !ws || reduction < 0 || reduction > 2 ||
       (dt != ACC_F32 && dt != ACC_BF16) || (top_dt != ACC_F32 && top_dt != ACC_BF16))
     return ACC_EBADARG;
-  if (((uintptr_t)save | (uintptr_t)ws) & 15) return ACC_EBADARG;
+  if (((uintptr_t)save | (uintptr_t)ws | (uintptr_t)z) & 15) return ACC_EBADARG;
   if (dz && (reduction == 0 || !accunet_distill_fused(B, S, V, dt) ||
              (((uintptr_t)z ^ (uintptr_t)dz) & 15)))
     return ACC_EBADARG;

@@ -5,8 +5,7 @@
 // read and written class by class. Rows up to DTR_WAVE_V classes take one wave each, longer
 // ones blocks of 256 threads, several blocks a row where the rows alone do not fill the
 // card. Where one block has a whole row, the gradient for an upstream of 1 is written by the
-// same kernel: the row's second read comes from the caches (rows in flight are kept to about
-// 128 MB by the number of threads a row gets), so the logits cross the memory bus once.
+// same kernel (short rows: from registers).
 // With a remaining mass the listed classes are kept out of the sum by a byte of marks
 // per vector in LDS (one read per vector, nearly always zero).
 #include <type_traits>
@@ -64,30 +63,52 @@ ACC_DEV void dt_load(const T* z, int off, int V, int q, float (&v)[DtVec<T>::N])
 template <typename T>
 ACC_DEV int dt_offset(const T* p) { return (int)(((uintptr_t)p & 15) / sizeof(T)); }
 
+// marks of the listed classes of vectors [qc, qe), one byte a vector, by threads t of NT
+template <int N, int NT>
+ACC_DEV void dt_marks(unsigned* mark, int qc, int qe, const int* id, int K, int off, int t) {
+  auto sync = [&]() {
+    if constexpr (NT > 64) __syncthreads();
+    else dt_wave_lds();
+  };
+  sync();
+  for (int w = t; w < (qe - qc + 3) / 4; w += NT) mark[w] = 0u;
+  sync();
+  for (int k = t; k < K; k += NT) {
+    const int j = id[k];
+    const int q = (j + off) / N - qc;
+    if (j >= 0 && q >= 0 && q < qe - qc)
+      atomicOr(&mark[q >> 2], 1u << ((q & 3) * 8 + (j + off) % N));
+  }
+  sync();
+}
+ACC_DEV unsigned dt_mark(const unsigned* mark, int q) {
+  return reinterpret_cast<const unsigned char*>(mark)[q];
+}
+
+// gradient vector q of a row: whole, or class by class at the row's ends and around listed
+// classes (`bits`), which others write
+template <typename T, bool STREAM>
+ACC_DEV void dt_put(T* dr, int off, int V, int q, unsigned bits, const float (&v)[DtVec<T>::N]) {
+  constexpr int N = DtVec<T>::N;
+  const int j = q * N - off;
+  if (j >= 0 && j + N <= V && bits == 0u) {
+    DtVec<T>::template st<STREAM>(dr + j, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (j + e >= 0 && j + e < V && !((bits >> e) & 1u)) st1(dr + j + e, v[e]);
+  }
+}
+
 // (m, s) over vectors [q0, q1) of a row, by threads t of NT; `mark`: DTR_CHUNK bytes
 template <typename T, bool REST, int NT>
 ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id, int K, int t,
                        unsigned* mark, float c, float& m, float& s) {
   constexpr int N = DtVec<T>::N;
-  constexpr int U = 4;
-  auto sync = [&]() {
-    if constexpr (NT > 64) __syncthreads();
-    else dt_wave_lds();
-  };
+  constexpr int U = sizeof(T) == 4 ? 4 : 2;  // vectors in flight a thread
   for (int qc = q0; qc < q1; qc += DTR_CHUNK) {
     const int qe = min(q1, qc + DTR_CHUNK);
-    if (REST) {
-      sync();
-      for (int w = t; w < (qe - qc + 3) / 4; w += NT) mark[w] = 0u;
-      sync();
-      for (int k = t; k < K; k += NT) {
-        const int j = id[k];
-        const int q = (j + off) / N - qc;
-        if (j >= 0 && q >= 0 && q < qe - qc)
-          atomicOr(&mark[q >> 2], 1u << ((q & 3) * 8 + (j + off) % N));
-      }
-      sync();
-    }
+    if (REST) dt_marks<N, NT>(mark, qc, qe, id, K, off, t);
     for (int q = qc + t; q < qe; q += NT * U) {
       float v[U][N];
 #pragma unroll
@@ -100,7 +121,7 @@ ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (q + u * NT >= qe) continue;
-          const unsigned bits = reinterpret_cast<const unsigned char*>(mark)[q + u * NT - qc];
+          const unsigned bits = dt_mark(mark, q + u * NT - qc);
           if (bits)
 #pragma unroll
             for (int e = 0; e < N; ++e) v[u][e] = (bits >> e) & 1u ? -INFINITY : v[u][e];
@@ -125,15 +146,16 @@ ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id
 }
 
 // One wave: the row's state and loss from (m, s) over the streamed classes.
-template <typename T>
-ACC_DEV float4 dt_finish_row(const T* z, const int* id, const float* p, int K, float m, float s,
+// zk(k): the logit of listed entry k.
+template <typename F>
+ACC_DEV float4 dt_finish_row(F zk, const int* id, const float* p, int K, float m, float s,
                            float rest, bool has_rest, float h, float c, float scale, int lane,
                            float4* state, float* rowloss, double* part) {
   const float mr = m, sr = s;
   if (has_rest) {
     float lm = -INFINITY, ls = 0.f;
     for (int k = lane; k < K; k += 64)
-      if (id[k] >= 0) dt_join(lm, ls, ld1(z + id[k]), 1.f, c);
+      if (id[k] >= 0) dt_join(lm, ls, zk(k), 1.f, c);
     dt_wave_join(lm, ls, c);
     dt_join(m, s, lm, ls, c);
   }
@@ -142,7 +164,7 @@ ACC_DEV float4 dt_finish_row(const T* z, const int* id, const float* p, int K, f
   for (int k = lane; k < K; k += 64) {
     const float pk = p[k];
     if (id[k] >= 0 && !(pk == 0.f))
-      dot += pk * (__builtin_fmaf(ld1(z + id[k]), c, -o.M) - o.log2S);
+      dot += pk * (__builtin_fmaf(zk(k), c, -o.M) - o.log2S);
   }
   dot = dt_wave_sum(dot);
   if (has_rest && !(rest == 0.f)) dot += rest * ((dt_ref(mr, c) - o.M) + log2f(sr) - o.log2S);
@@ -164,6 +186,12 @@ ACC_DEV void dt_empty_row(int lane, float4* state, float* rowloss, double* part)
   }
 }
 
+template <typename T>
+ACC_DEV void dt_put_listed(const T* zr, T* dr, int j, float p, const float4& st, float c,
+                           float gs) {
+  st1(dr + j, gs * (dt_exp2(__builtin_fmaf(ld1(zr + j), c, -st.z)) * st.w - p));
+}
+
 // Gradient of vectors [q0, q1) of a row by threads t of NT: every class as not listed, then,
 // behind a barrier, the listed classes over it. `dr` has z's alignment (checked by the host).
 // STREAM: stored past the caches.
@@ -171,7 +199,7 @@ template <typename T, int NT, bool STREAM>
 ACC_DEV void dt_gradient(const T* zr, T* dr, int off, int V, int q0, int q1, const int* id,
                          const float* p, int K, int t, const float4& st, float c, float gs) {
   constexpr int N = DtVec<T>::N;
-  constexpr int U = 4;
+  constexpr int U = sizeof(T) == 4 ? 4 : 2;
   const bool live = !(st.w == DT_EMPTY);
   const float cu = st.y * gs;
   for (int q = q0 + t; q < q1; q += NT * U) {
@@ -187,14 +215,7 @@ ACC_DEV void dt_gradient(const T* zr, T* dr, int off, int V, int q0, int q1, con
 #pragma unroll
       for (int e = 0; e < N; ++e)
         v[u][e] = live ? dt_exp2(__builtin_fmaf(v[u][e], c, -st.x)) * cu : 0.f;
-      const int j = (q + u * NT) * N - off;
-      if (j >= 0 && j + N <= V) {
-        DtVec<T>::template st<STREAM>(dr + j, v[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (j + e >= 0 && j + e < V) st1(dr + j + e, v[u][e]);
-      }
+      dt_put<T, STREAM>(dr, off, V, q + u * NT, 0u, v[u]);
     }
   }
   if (!live) return;  // the same for the whole row
@@ -204,8 +225,7 @@ ACC_DEV void dt_gradient(const T* zr, T* dr, int off, int V, int q0, int q1, con
   for (int k = t; k < K; k += NT) {
     const int j = id[k];
     const int q = (j + off) / N;
-    if (j >= 0 && q >= q0 && q < q1)
-      st1(dr + j, gs * (dt_exp2(__builtin_fmaf(ld1(zr + j), c, -st.z)) * st.w - p[k]));
+    if (j >= 0 && q >= q0 && q < q1) dt_put_listed(zr, dr, j, p[k], st, c, gs);
   }
 }
 
@@ -221,11 +241,14 @@ ACC_DEV void dt_small_loss(const DtArgs& a, double* red) {
   }
 }
 
-// short rows: one wave a row, everything in one pass
-template <typename T, bool REST>
+// short rows: one wave a row, NQ vectors a lane in registers. The exponentials are relative
+// to the largest streamed class, which is the gradient's reference too (mu), so each is
+// computed once: dz = e * cu. 65536 x 2000 bf16: see the figure at the launch.
+template <typename T, bool REST, int NQ>
 __global__ void __launch_bounds__(256)
 distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
-  __shared__ unsigned mark[4][(DTR_WAVE_V / 4 + 2 + 3) / 4];
+  constexpr int N = DtVec<T>::N;
+  __shared__ unsigned mark[4][NQ * 16];
   __shared__ double red[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long row = blockIdx.x * 4L + wave;
@@ -234,65 +257,162 @@ distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
     float* rl = a.none ? a.loss + row : nullptr;
     const float2 te = a.tea[row];
     const T* zr = (const T*)a.z + row * V;
-    const int off = dt_offset(zr), nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
-    float4 st = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
+    T* dr = (T*)a.dz + row * V;
+    const int* id = a.id + row * K;
+    const float* p = a.p + row * K;
+    const int off = dt_offset(zr), nq = (off + V + N - 1) / N;
     if (te.y == 0.f) {
       dt_empty_row(lane, a.state + row, rl, &red[wave]);
+      if (a.dz) {
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = 0.f;
+        for (int q = lane; q < nq; q += 64) dt_put<T, false>(dr, off, V, q, 0u, v);
+      }
     } else {
-      float m = -INFINITY, s = 0.f;
-      dt_stream<T, REST, 64>(zr, off, V, 0, nq, a.id + row * K, K, lane, mark[wave], a.c, m, s);
-      dt_wave_join(m, s, a.c);
-      st = dt_finish_row(zr, a.id + row * K, a.p + row * K, K, m, s, REST ? a.rest[row] : 0.f, REST,
-                         te.x, a.c, a.scale, lane, a.state + row, rl, &red[wave]);
+      float v[NQ][N];
+#pragma unroll
+      for (int u = 0; u < NQ; ++u) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u][e] = -INFINITY;
+        if (u * 64 + lane < nq) dt_load(zr, off, V, u * 64 + lane, v[u]);
+      }
+      if (REST || a.dz) dt_marks<N, 64>(mark[wave], 0, nq, id, K, off, lane);
+      unsigned bits[NQ];
+#pragma unroll
+      for (int u = 0; u < NQ; ++u) {
+        bits[u] = (REST || a.dz) && u * 64 + lane < nq ? dt_mark(mark[wave], u * 64 + lane) : 0u;
+        if (REST && bits[u])
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[u][e] = (bits[u] >> e) & 1u ? -INFINITY : v[u][e];
+      }
+      float m = v[0][0];
+#pragma unroll
+      for (int u = 0; u < NQ; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, v[u][e]);
+      m = dt_wave_max(m);
+      const float ref = dt_ref(m, a.c);
+      float s = 0.f;
+#pragma unroll
+      for (int u = 0; u < NQ; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          v[u][e] = dt_exp2(__builtin_fmaf(v[u][e], a.c, -ref));
+          s += v[u][e];
+        }
+      s = dt_wave_sum(s);
+      const float4 st = dt_finish_row([&](int k) { return ld1(zr + id[k]); }, id, p, K, m, s,
+                                      REST ? a.rest[row] : 0.f, REST, te.x, a.c, a.scale, lane,
+                                      a.state + row, rl, &red[wave]);
+      if (a.dz) {
+        const float gs = dt_scale(g, row), cu = st.y * gs;
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+          if (u * 64 + lane >= nq) continue;
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[u][e] *= cu;
+          dt_put<T, false>(dr, off, V, u * 64 + lane, bits[u], v[u]);
+        }
+        for (int k = lane; k < K; k += 64)
+          if (id[k] >= 0) dt_put_listed(zr, dr, id[k], p[k], st, a.c, gs);
+      }
     }
     if (lane == 0) {
       a.part[row] = red[wave];
       if (a.applied) a.applied[row] = 1.f;
     }
-    if (a.dz)
-      dt_gradient<T, 64, false>(zr, (T*)a.dz + row * V, off, V, 0, nq, a.id + row * K,
-                                a.p + row * K, K, lane, st, a.c, dt_scale(g, row));
   }
   dt_small_loss(a, red);
 }
 
-// long rows, one block each: the sum, the row's loss and the gradient
+// long rows, one block each: the sum, the row's loss and the gradient. The listed entries
+// are fetched at the start, beside the stream, and marked in LDS for the whole row where it
+// has at most DTR_CHUNK vectors: the gradient then goes around them and they are written
+// without waiting for it.
+// The gradient's second read of the row finds little of it in the caches: the rows in
+// flight are larger than the L2 (4096 x 128000 bf16: 522 us, three passes at 6 TB/s). Held
+// in registers instead (64 a thread for the row, one block a CU) it took 592-860 us: sums,
+// barriers and stores of one row then stand one behind another on each CU.
 template <typename T, bool REST, int NT, bool STREAM>
-__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8)))
+__global__ void __launch_bounds__(NT)
 distill_rows_fused_kernel(const DtArgs a, const DtScale g) {
-  __shared__ unsigned mark[REST ? DTR_CHUNK / 4 : 1];
+  constexpr int N = DtVec<T>::N;
+  __shared__ unsigned mark[DTR_CHUNK / 4];
   __shared__ float2 red[NT / 64];
   __shared__ float4 rs;
+  __shared__ int lid[DT_MAX_K];
+  __shared__ float lp[DT_MAX_K], lz[DT_MAX_K];
   const long row = blockIdx.x;
   const int t = threadIdx.x, V = a.V, K = a.K;
   const T* zr = (const T*)a.z + row * V;
-  const int off = dt_offset(zr), nq = (off + V + DtVec<T>::N - 1) / DtVec<T>::N;
+  T* dr = (T*)a.dz + row * V;
+  const int off = dt_offset(zr), nq = (off + V + N - 1) / N;
   float* rl = a.none ? a.loss + row : nullptr;
   const float2 te = a.tea[row];
-  float4 st = make_float4(0.f, 0.f, 0.f, DT_EMPTY);
+  if (t == 0 && a.applied) a.applied[row] = 1.f;
   if (te.y == 0.f) {
     dt_empty_row(t, a.state + row, rl, a.part + row);
-  } else {
-    float m = -INFINITY, s = 0.f;
-    dt_stream<T, REST, NT>(zr, off, V, 0, nq, a.id + row * K, K, t, mark, a.c, m, s);
-    dt_wave_join(m, s, a.c);
-    if ((t & 63) == 0) red[t >> 6] = make_float2(m, s);
-    __syncthreads();
-    if (t < 64) {
-      m = red[0].x;
-      s = red[0].y;
-      for (int w = 1; w < NT / 64; ++w) dt_join(m, s, red[w].x, red[w].y, a.c);
-      st = dt_finish_row(zr, a.id + row * K, a.p + row * K, K, m, s, REST ? a.rest[row] : 0.f, REST,
-                         te.x, a.c, a.scale, t, a.state + row, rl, a.part + row);
-      if (t == 0) rs = st;
+    if (a.dz) {
+      float v[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = 0.f;
+      for (int q = t; q < nq; q += NT) dt_put<T, STREAM>(dr, off, V, q, 0u, v);
     }
-    __syncthreads();
-    st = rs;
+    return;
   }
-  if (t == 0 && a.applied) a.applied[row] = 1.f;
-  if (a.dz)
-    dt_gradient<T, NT, STREAM>(zr, (T*)a.dz + row * V, off, V, 0, nq, a.id + row * K, a.p + row * K,
-                               K, t, st, a.c, dt_scale(g, row));
+  int my = -1;  // K <= DT_MAX_K <= NT: an entry a thread
+  float mp = 0.f, mz = 0.f;
+  if (t < K) {
+    my = a.id[row * K + t];
+    mp = a.p[row * K + t];
+    mz = my >= 0 ? ld1(zr + my) : 0.f;
+    lid[t] = my;
+  }
+  __syncthreads();
+  const bool one = nq <= DTR_CHUNK;
+  if (one && !REST && a.dz) dt_marks<N, NT>(mark, 0, nq, lid, K, off, t);
+  float m = -INFINITY, s = 0.f;
+  dt_stream<T, REST, NT>(zr, off, V, 0, nq, lid, K, t, mark, a.c, m, s);
+  dt_wave_join(m, s, a.c);
+  if ((t & 63) == 0) red[t >> 6] = make_float2(m, s);
+  if (t < K) {
+    lp[t] = mp;
+    lz[t] = mz;
+  }
+  __syncthreads();
+  if (t < 64) {
+    m = red[0].x;
+    s = red[0].y;
+    for (int w = 1; w < NT / 64; ++w) dt_join(m, s, red[w].x, red[w].y, a.c);
+    const float4 st = dt_finish_row([&](int k) { return lz[k]; }, lid, lp, K, m, s,
+                                    REST ? a.rest[row] : 0.f, REST, te.x, a.c, a.scale, t,
+                                    a.state + row, rl, a.part + row);
+    if (t == 0) rs = st;
+  }
+  if (!a.dz) return;
+  __syncthreads();
+  const float4 st = rs;
+  const float gs = dt_scale(g, row), cu = st.y * gs;
+  if (!one) {
+    dt_gradient<T, NT, STREAM>(zr, dr, off, V, 0, nq, lid, lp, K, t, st, a.c, gs);
+    return;
+  }
+  if (my >= 0) dt_put_listed(zr, dr, my, mp, st, a.c, gs);
+  constexpr int U = sizeof(T) == 4 ? 4 : 2;
+  for (int q = t; q < nq; q += NT * U) {
+    float v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * NT < nq) dt_load(zr, off, V, q + u * NT, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (q + u * NT >= nq) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[u][e] = dt_exp2(__builtin_fmaf(v[u][e], a.c, -st.x)) * cu;
+      dt_put<T, STREAM>(dr, off, V, q + u * NT, dt_mark(mark, q + u * NT), v[u]);
+    }
+  }
 }
 
 // long rows, several blocks each: block (row, y) streams the y-th run into ms[row][y]
@@ -338,7 +458,9 @@ distill_rows_finish_kernel(const DtArgs a, int runs) {
         dt_join(m, s, v.x, v.y, a.c);
       }
       dt_wave_join(m, s, a.c);
-      dt_finish_row((const T*)a.z + row * V, a.id + row * K, a.p + row * K, K, m, s,
+      const T* zr = (const T*)a.z + row * V;
+      const int* id = a.id + row * K;
+      dt_finish_row([&](int k) { return ld1(zr + id[k]); }, id, a.p + row * K, K, m, s,
                     REST ? a.rest[row] : 0.f, REST, te.x, a.c, a.scale, lane, a.state + row, rl,
                     &red[wave]);
     }
@@ -396,15 +518,23 @@ void dt_rows_forward(const DtArgs& a, int dt, hipStream_t st) {
       constexpr bool REST = decltype(rtag)::value;
       const dim3 g4((unsigned)((a.rows + 3) / 4));
       if (a.V <= DTR_WAVE_V) {
-        hipLaunchKernelGGL((distill_rows_wave_kernel<Z, REST>), g4, dim3(256), 0, st, a, g);
+        // vectors a row has at most: a row of whole vectors starts at an aligned address
+        constexpr int N = 16 / sizeof(Z);
+        const int nq = (a.V + (a.V % N ? 2 * N - 2 : 0)) / N;
+        auto nt = [&](auto tag2) {
+          constexpr int NQ = decltype(tag2)::value;
+          hipLaunchKernelGGL((distill_rows_wave_kernel<Z, REST, NQ>), g4, dim3(256), 0, st, a, g);
+        };
+        if (nq <= 64) nt(std::integral_constant<int, 1>{});
+        else if (nq <= 128) nt(std::integral_constant<int, 2>{});
+        else if (nq <= 256) nt(std::integral_constant<int, 4>{});
+        else nt(std::integral_constant<int, 8>{});
         return;
       }
       const int runs = dt_rows_runs(a.rows, a.V, dt);
       if (runs == 1) {
-        // threads a row: a CU's 2048 hold at most 512 KB of rows
-        const long bytes = (long)a.V * sizeof(Z);
         const dim3 grid((unsigned)a.rows);
-        auto nt = [&](auto ntag) {
+        auto run = [&](auto ntag) {
           constexpr int NT = decltype(ntag)::value;
           if (dt_large<Z>(a))
             hipLaunchKernelGGL((distill_rows_fused_kernel<Z, REST, NT, true>), grid, dim3(NT), 0,
@@ -413,9 +543,13 @@ void dt_rows_forward(const DtArgs& a, int dt, hipStream_t st) {
             hipLaunchKernelGGL((distill_rows_fused_kernel<Z, REST, NT, false>), grid, dim3(NT), 0,
                                st, a, g);
         };
-        if (bytes <= (64 << 10)) nt(std::integral_constant<int, 256>{});
-        else if (bytes <= (128 << 10)) nt(std::integral_constant<int, 512>{});
-        else nt(std::integral_constant<int, 1024>{});
+        // threads a row: 2048 a CU then hold 512 KB of rows at most; 4096 x 128000 bf16 took
+        // 522 us with 1024 threads, 555 with 512, 650 with 256, 16384 x 32000 took 617 us
+        // with 1024, 531 with 512, 553 with 256
+        const long bytes = (long)a.V * sizeof(Z);
+        if (bytes <= (64 << 10)) run(std::integral_constant<int, 256>{});
+        else if (bytes <= (128 << 10)) run(std::integral_constant<int, 512>{});
+        else run(std::integral_constant<int, 1024>{});
         return;
       }
       hipLaunchKernelGGL((distill_rows_sum_kernel<Z, REST>), dim3((unsigned)a.rows, runs),
