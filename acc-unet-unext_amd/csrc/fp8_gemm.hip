@@ -60,8 +60,22 @@ struct Fp8GemmArgs {
   float* slab;  // split: [splits][M][N] partial sums
   long M, N;
   int KP, SP, kt_per;  // k-tiles per split (a multiple of 4)
-  int tiles_n, vec;
+  int tiles_m, tiles_n, vec;
 };
+
+// Tile of a block. Blocks go to the 8 XCDs in turn, each with an L2 of its own: XCD x takes
+// the x-th eighth of the tiles, in groups of 8 rows of tiles walked column by column, so
+// that what runs together on an XCD shares its operands. false past the last tile.
+ACC_DEV bool fp8_tile(const Fp8GemmArgs& g, int& mt, int& nt) {
+  const int total = g.tiles_m * g.tiles_n, per = (total + 7) / 8;
+  const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (t >= total || (int)(blockIdx.x >> 3) >= per) return false;
+  const int group = t / (8 * g.tiles_n), rows = min(8, g.tiles_m - group * 8);
+  const int in = t - group * 8 * g.tiles_n;
+  mt = group * 8 + in % rows;
+  nt = in / rows;
+  return true;
+}
 
 template <typename T>
 ACC_DEV void fp8_store4(T* p, const float (&v)[4], int n, bool vec) {
@@ -74,50 +88,66 @@ ACC_DEV void fp8_store4(T* p, const float (&v)[4], int n, bool vec) {
   }
 }
 
-template <typename T, bool SPLIT, bool WIDE>
-__global__ void __launch_bounds__(256, 2)
+// WM x WN waves, TM x TN fragments of 16 x 16 each. 128 x 128 tiles (2 x 2 waves of 4 x 4)
+// read 64 KB of fragments a k-tile from LDS for 512 cycles of matrix work, which is more than
+// LDS delivers beside the copies; 256 x 256 tiles (2 x 4 waves of 8 x 4) read 192 KB for
+// 2048 cycles, one block a CU. 16384 x 4096 x 4096 in bf16: 272 us (2.02 PFLOP/s) with
+// 128 x 128, 242 us (2.27) with 256 x 256; fp32 outputs 485 and 422 us (1.30); 4096 x 4096 x
+// 16384 211 us (2.60).
+template <typename T, bool SPLIT, bool WIDE, int WM, int WN, int TM, int TN>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
 fp8_gemm_kernel(const Fp8GemmArgs g) {
-  constexpr int BM = 128, BN = 128;
+  constexpr int BM = WM * TM * 16, BN = WN * TN * 16, NW = WM * WN;
+  constexpr int IA = BM / 8 / NW, IB = BN / 8 / NW;  // copies of 8 rows a wave
+  static_assert(BM + BN == 64 * NW && BM % 64 == 0, "one scale dword a thread");
   __shared__ __attribute__((aligned(1024))) unsigned char sA[2][BM * 128];
   __shared__ __attribute__((aligned(1024))) unsigned char sB[2][BN * 128];
   __shared__ __attribute__((aligned(1024))) unsigned sS[2][BM + BN];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wm = wave & 1, wn = wave >> 1;
-  const long m0 = (long)(blockIdx.x / g.tiles_n) * BM;
-  const long n0 = (long)(blockIdx.x % g.tiles_n) * BN;
+  const int wm = wave % WM, wn = wave / WM;
+  int mt, nt;
+  if (!fp8_tile(g, mt, nt)) return;
+  const long m0 = (long)mt * BM, n0 = (long)nt * BN;
   const int kt0 = SPLIT ? blockIdx.z * g.kt_per : 0;
   const int kt1 = SPLIT ? min(g.KP / 128, kt0 + g.kt_per) : g.KP / 128;
 
-  const unsigned char *pa[4], *pb[4];
+  const unsigned char *pa[IA], *pb[IB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = wave * 32 + i * 8 + (lane >> 3);
-    const int ch = (lane & 7) ^ ((r >> 1) & 7);
-    pa[i] = g.a + min(m0 + r, g.M - 1) * g.KP + ch * 16 + (long)kt0 * 128;
-    pb[i] = g.b + min(n0 + r, g.N - 1) * g.KP + ch * 16 + (long)kt0 * 128;
+  for (int i = 0; i < IA; ++i) {
+    const int r = (wave * IA + i) * 8 + (lane >> 3);
+    pa[i] = g.a + min(m0 + r, g.M - 1) * g.KP + ((lane & 7) ^ ((r >> 1) & 7)) * 16 + (long)kt0 * 128;
   }
-  const unsigned char* ps = wave < 2 ? g.sa + min(m0 + t, g.M - 1) * g.SP
-                                     : g.sb + min(n0 + t - BM, g.N - 1) * g.SP;
+#pragma unroll
+  for (int i = 0; i < IB; ++i) {
+    const int r = (wave * IB + i) * 8 + (lane >> 3);
+    pb[i] = g.b + min(n0 + r, g.N - 1) * g.KP + ((lane & 7) ^ ((r >> 1) & 7)) * 16 + (long)kt0 * 128;
+  }
+  const unsigned char* ps = wave < BM / 64 ? g.sa + min(m0 + t, g.M - 1) * g.SP
+                                           : g.sb + min(n0 + t - BM, g.N - 1) * g.SP;
   auto stage = [&](int kt) {
     const int buf = (kt - kt0) & 1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fp8_dma16(pa[i], fp8_lds_addr(&sA[buf][(wave * 32 + i * 8) * 128]));
-      fp8_dma16(pb[i], fp8_lds_addr(&sB[buf][(wave * 32 + i * 8) * 128]));
+    for (int i = 0; i < IA; ++i) {
+      fp8_dma16(pa[i], fp8_lds_addr(&sA[buf][(wave * IA + i) * 1024]));
       pa[i] += 128;
+    }
+#pragma unroll
+    for (int i = 0; i < IB; ++i) {
+      fp8_dma16(pb[i], fp8_lds_addr(&sB[buf][(wave * IB + i) * 1024]));
       pb[i] += 128;
     }
     if (((kt - kt0) & 3) == 0) fp8_dma4(ps + kt, fp8_lds_addr(&sS[((kt - kt0) >> 2) & 1][wave * 64]));
   };
 
-  v4f acc[4][4];
+  v4f acc[TM][TN];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-  unsigned sa[4], sb[4];
+    for (int j = 0; j < TN; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  unsigned sa[TM], sb[TN];
   const int l15 = lane & 15, kg = lane >> 4;
+  const int ra = wm * TM * 16 + l15, rb = wn * TN * 16 + l15;
   auto frag = [&](const unsigned char* tile, int r) {
     const int sw = (r >> 1) & 7;
     const v4i lo = *reinterpret_cast<const v4i*>(tile + r * 128 + ((2 * kg) ^ sw) * 16);
@@ -135,57 +165,57 @@ fp8_gemm_kernel(const Fp8GemmArgs g) {
     if (q == 0) {
       const unsigned* sc = sS[((kt - kt0) >> 2) & 1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sa[i] = sc[wm * 64 + i * 16 + l15];
-        sb[i] = sc[BM + wn * 64 + i * 16 + l15];
-      }
-    }
-    v8i fa[4], fb[4];
+      for (int i = 0; i < TM; ++i) sa[i] = sc[ra + i * 16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[i] = frag(sA[buf], wm * 64 + i * 16 + l15);
-      fb[i] = frag(sB[buf], wn * 64 + i * 16 + l15);
+      for (int j = 0; j < TN; ++j) sb[j] = sc[BM + rb + j * 16];
     }
+    v8i fb[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[j] = frag(sB[buf], rb + j * 16);
     if constexpr (WIDE) {
+      v8i fa[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = frag(sA[buf], ra + i * 16);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v8b wb[4];
+        v8b wb[TN];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < TN; ++j)
           wb[j] = fp8_widen(fb[j][2 * k], fb[j][2 * k + 1], __uint_as_float((sb[j] & 255u) << 23));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < TM; ++i) {
           const v8b wa =
               fp8_widen(fa[i][2 * k], fa[i][2 * k + 1], __uint_as_float((sa[i] & 255u) << 23));
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < TN; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], wa, acc[i][j], 0, 0, 0);
         }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < TM; ++i) {
+        const v8i fa = frag(sA[buf], ra + i * 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < TN; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              fb[j], fa[i], acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+              fb[j], fa, acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sa[i] >>= 8;
-      sb[i] >>= 8;
-    }
+    for (int i = 0; i < TM; ++i) sa[i] >>= 8;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sb[j] >>= 8;
   }
 
   // lane: m = l15 of the fragment, n = 4 kg .. + 3
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long m = m0 + wm * 64 + i * 16 + l15;
+  for (int i = 0; i < TM; ++i) {
+    const long m = m0 + ra + i * 16;
     if (m >= g.M) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long n = n0 + wn * 64 + j * 16 + kg * 4;
-      const int left = (int)min(4L, g.N - n);
+    for (int j = 0; j < TN; ++j) {
+      const long n = n0 + wn * TN * 16 + j * 16 + kg * 4;
+      const int left = (int)max(0L, min(4L, g.N - n));
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
@@ -236,8 +266,11 @@ extern "C" int accunet_fp8_gemm(const void* a, const void* sa, const void* b, co
                                 const float* bias, void* c, float* ws, size_t ws_elems, long M,
                                 long N, long K, int cdt, void* stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K > (1L << 30)) return ACC_EBADSHAPE;
-  const long tm = (M + 127) / 128, tn = (N + 127) / 128;
-  if (tn > 0x7fffffffL || tm * tn > 0x7fffffffL) return ACC_EBADSHAPE;
+  // 256 x 256 tiles where they alone give every CU one, 128 x 128 else
+  const bool big = ((M + 255) / 256) * ((N + 255) / 256) >= 256;
+  const int bt = big ? 256 : 128;
+  const long tm = (M + bt - 1) / bt, tn = (N + bt - 1) / bt;
+  if (tn > 0x7fffffffL || tm * tn > 0x7ffffff0L) return ACC_EBADSHAPE;
   if (!a || !sa || !b || !sb || !c) return ACC_EBADARG;
   if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)sa | (uintptr_t)sb) & 3) return ACC_EBADARG;
   if (ws_elems < accunet_fp8_gemm_ws_elems(M, N, K)) return ACC_EBADARG;
@@ -246,22 +279,26 @@ extern "C" int accunet_fp8_gemm(const void* a, const void* sa, const void* b, co
   g.b = (const unsigned char*)b; g.sb = (const unsigned char*)sb;
   g.c = c; g.bias = bias; g.slab = ws;
   g.M = M; g.N = N; g.KP = (int)fp8_pad(K); g.SP = (int)fp8_scale_pitch(K);
-  g.tiles_n = (int)tn;
+  g.tiles_m = (int)tm; g.tiles_n = (int)tn;
   const int splits = fp8_splits(M, N, K);
   const int quads = (g.KP / 128 + 3) / 4;
   g.kt_per = (quads + splits - 1) / splits * 4;
   hipStream_t st = (hipStream_t)stream;
   const int rc = with_dt(cdt, [&](auto tag) {
     using T = decltype(tag);
-    const dim3 grid((unsigned)(tm * tn), 1, splits);
+    constexpr bool WIDE = sizeof(T) == 4;
+    const dim3 grid((unsigned)((tm * tn + 7) / 8 * 8), 1, splits);
     if (splits > 1) {
       g.vec = N % 4 == 0 && ((uintptr_t)ws & 15) == 0;
-      hipLaunchKernelGGL((fp8_gemm_kernel<T, true, sizeof(T) == 4>), grid, dim3(256), 0, st, g);
+      hipLaunchKernelGGL((fp8_gemm_kernel<T, true, WIDE, 2, 2, 4, 4>), grid, dim3(256), 0, st, g);
       hipLaunchKernelGGL(fp8_join_kernel<T>, dim3((unsigned)((M * N + 255) / 256)), dim3(256), 0,
                          st, ws, splits, bias, (T*)c, M * N, N);
     } else {
       g.vec = N % 4 == 0 && ((uintptr_t)c & (4 * sizeof(T) - 1)) == 0;
-      hipLaunchKernelGGL((fp8_gemm_kernel<T, false, sizeof(T) == 4>), grid, dim3(256), 0, st, g);
+      if (big)
+        hipLaunchKernelGGL((fp8_gemm_kernel<T, false, WIDE, 2, 4, 8, 4>), grid, dim3(512), 0, st, g);
+      else
+        hipLaunchKernelGGL((fp8_gemm_kernel<T, false, WIDE, 2, 2, 4, 4>), grid, dim3(256), 0, st, g);
     }
   });
   if (rc != ACC_OK) return rc;
