@@ -161,17 +161,20 @@ _SIGS = {
     "accunet_distill_fused": [L, L, I, I],
     "accunet_distill_fwd": [P, P, I, P, I, P, P, I, P, P, S, P, S, L, L, I, I, F, F, I, P],
     "accunet_distill_bwd": [P, P, S, P, I, I, P, L, L, I, I, F, F, I, P],
-    "accunet_fp8_sum_ws_elems": [L, I],
-    "accunet_fp8_quantize": [P, I, P, P, P, P, P, P, S, L, I, I, P],
-    "accunet_fp8_gemm_ws_elems": [L, L, L],
-    "accunet_fp8_gemm": [P, P, P, P, P, P, P, S, L, L, L, I, P],
+    "accunet_fp8_quantize": [P, I, P, P, P, P, L, I, I, P],
+    "accunet_fp8_linear_save_bytes": [L, L, L, I, I],
+    "accunet_fp8_linear_ws_bytes": [L, L, L, I],
+    "accunet_fp8_linear_bwd_ws_bytes": [L, L, L, I, I, I],
+    "accunet_fp8_linear_fwd": [P, P, P, P, P, P, I, I, P, S, P, S, L, L, L, I, P],
+    "accunet_fp8_linear_bwd": [P, P, I, I, P, P, P, P, P, P, S, L, L, L, I, P],
 }
 # entry points returning a size/count rather than a status
 _SIZE_FNS = {"accunet_bn_bwd_ws_elems", "accunet_bn_bwd_part_ws_elems", "accunet_dw3x3_wgrad_ws", "accunet_se_save_elems", "accunet_se_ws_elems",
              "accunet_head_ws_elems", "accunet_loss_ws_elems", "accunet_dwconvk_wgrad_ws",
              "accunet_dwconvk_dgrad_ws", "accunet_blocknorm_ws_elems",
              "accunet_distill_save_bytes", "accunet_distill_ws_bytes",
-             "accunet_fp8_sum_ws_elems", "accunet_fp8_gemm_ws_elems"}
+             "accunet_fp8_linear_save_bytes", "accunet_fp8_linear_ws_bytes",
+             "accunet_fp8_linear_bwd_ws_bytes"}
 
 _LL_FNS = {"accunet_abi_hash", "accunet_conv3x3_halo_launches"}
 HEADER = os.path.join(os.path.dirname(os.path.dirname(_HERE)), "include", "accunet.h")

@@ -64,13 +64,9 @@ class _BlockNormFn(torch.autograd.Function):
         dg = torch.empty_like(g) if g is not None else None
         dpar = torch.empty(5, C, dtype=torch.float32, device=x.device)
         kern.blocknorm_bwd(x, f, w1, b1, s, g, w2, layer, stats, dr, dh, dx, df, dg, dpar, P, L, C)
-        need = ctx.needs_input_grad
-
-        def par(i, k):
-            return dpar[k] if need[i] else None
-
-        return (dx, df, par(2, 0), par(3, 1), par(4, 2), dg, par(6, 3), par(7, 4),
-                None, None, None, None)
+        par = [d if on else None for d, on in zip(dpar.unbind(0), ctx.needs_input_grad[2:5]
+                                                  + ctx.needs_input_grad[6:8])]
+        return (dx, df, par[0], par[1], par[2], dg, par[3], par[4], None, None, None, None)
 
 
 def _param(t, C, name, x):

@@ -12,7 +12,8 @@ gradients are quantised in blocks of 1 x 128 along the contracted axis, weights 
 
 Activations are float32 or bfloat16; weights, biases and their gradients are float32. An
 element that is not finite becomes NaN; scales stop at 2^-126 and 2^120. Non-contiguous
-inputs are copied (csrc/fp8.h, csrc/fp8_quant.hip, csrc/fp8_gemm.hip).
+inputs are copied. bf16 results come from the fp8 matrix instruction, fp32 results (and dw)
+from the bf16 one over the same values (csrc/fp8.h, csrc/fp8_gemm.hip, csrc/fp8_token.hip).
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ from . import kern
 from ._lib import AccError
 
 BLOCK = 128
+_MAX_DIM = 1 << 22
 
 
 def _pad(n):
@@ -63,14 +65,6 @@ def _new(rows, cols, dev):
             torch.empty(rows, _pitch(cols), dtype=torch.uint8, device=dev))
 
 
-def _quantize(x, R, C, square=False, rows=True, cols=False, colsum=None):
-    """(q, s), (qt, st) of x [R, C]; the column sums into `colsum`."""
-    q, s = _new(R, C, x.device) if rows else (None, None)
-    qt, st = _new(C, R, x.device) if cols else (None, None)
-    kern.fp8_quantize(x, square, q, s, qt, st, colsum, R, C)
-    return (q, s), (qt, st)
-
-
 def quantize(x, square=False, transposed=False):
     """Fp8Blocks of x [R, C] (float32 or bfloat16): blocks of 1 x 128, with square=True of
     128 x 128 (weights). transposed=True keeps the transposed matrix too, which the
@@ -81,61 +75,51 @@ def quantize(x, square=False, transposed=False):
     if transposed and not square:
         raise ValueError("fp8.quantize: transposed needs square blocks")
     R, C = x.shape
-    (q, s), (qt, st) = _quantize(x.detach().contiguous(), R, C, square, cols=transposed)
+    if C > _MAX_DIM or (transposed and R > _MAX_DIM):
+        raise AccError(f"fp8.quantize: at most {_MAX_DIM} columns, got {tuple(x.shape)}")
+    q, s = _new(R, C, x.device)
+    qt, st = _new(C, R, x.device) if transposed else (None, None)
+    kern.fp8_quantize(x.detach().contiguous(), square, q, s, qt, st, R, C)
     t = Fp8Blocks(qt, st, C, R, True) if transposed else None
     return Fp8Blocks(q, s, R, C, square, t)
 
 
-def _gemm(a, b, M, N, K, bias, dtype):
-    c = torch.empty(M, N, dtype=dtype, device=a[0].device)
-    kern.fp8_gemm(a[0], a[1], b[0], b[1], bias, c, M, N, K)
-    return c
-
-
-def _forward(x, weight, bias, wq, N, need_x=False, need_w=False, wt=None):
-    """y, and what the gradients need: the transposed x and weight."""
+def _forward(x, weight, bias, wq, N, need_w=False, need_wt=False):
+    """y, and what the gradients need: the transposed x and (of a float weight) weight."""
     K = x.shape[-1]
     M = x.numel() // K
-    xt = (None, None)
-    if M:
-        xq, xt = _quantize(x, M, K, cols=need_w)
-    if weight is not None and (M or need_x):
-        wq, wt = _quantize(weight, N, K, square=True, cols=need_x)
-    y = _gemm(xq, wq, M, N, K, bias, x.dtype) if M else x.new_empty(0, N)
-    return y.view(*x.shape[:-1], N), xt, (wt if need_x else (None, None))
+    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    if M == 0:
+        return y, None
+    q, s = (None, None) if wq is None else (wq.q, wq.s)
+    return y, kern.fp8_linear_fwd(x, weight, q, s, bias, y, need_w, need_wt, M, N, K)
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, wq, wt, N):
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        y, xt, wt = _forward(x, weight, bias, wq, N, need_x, need_w, wt)
-        ctx.save_for_backward(*xt, *wt)
+    def forward(ctx, x, weight, bias, wq, N):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        need_wt = need_x and weight is not None
+        y, save = _forward(x, weight, bias, wq, N, need_w, need_wt)
+        t = wq.t if need_x and wq is not None else None
+        ctx.save_for_backward(save, *((t.q, t.s) if t is not None else (None, None)))
         K = x.shape[-1]
-        ctx.cfg = (x.numel() // K, N, K, x.shape, x.dtype)
+        ctx.cfg = (x.numel() // K, N, K, x.shape, x.dtype, need_w, need_wt)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        qt, st, wqt, wst = ctx.saved_tensors
-        M, N, K, shape, dtype = ctx.cfg
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = dy.device
-        dx = dw = db = None
-        if M == 0:
-            return (torch.empty(shape, dtype=dtype, device=dev) if need_x else None,
-                    torch.zeros(N, K, device=dev) if need_w else None,
-                    torch.zeros(N, device=dev) if need_b else None, None, None, None)
-        dy = dy.contiguous()
-        db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
-        # the bias alone needs no quantised matrix, but shares the pass that makes one
-        rows, cols = _quantize(dy, M, N, rows=need_x or not need_w, cols=need_w, colsum=db)
-        if need_x:
-            dx = _gemm(rows, (wqt, wst), M, K, N, None, dtype).view(shape)
-        if need_w:
-            dw = _gemm(cols, (qt, st), N, K, M, None, torch.float32)
-        return dx, dw, db, None, None, None
+        save, wt, wts = ctx.saved_tensors
+        M, N, K, shape, dtype, need_w, need_wt = ctx.cfg
+        dev, f32 = dy.device, torch.float32
+        new = torch.empty if M else torch.zeros
+        dx = torch.empty(shape, dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = new(N, K, dtype=f32, device=dev) if need_w else None
+        db = new(N, dtype=f32, device=dev) if ctx.needs_input_grad[2] else None
+        if M:
+            kern.fp8_linear_bwd(dy.contiguous(), save, need_w, need_wt, wt, wts, dx, dw, db, M, N, K)
+        return dx, dw, db, None, None
 
 
 def linear(x, weight, bias=None):
@@ -148,7 +132,7 @@ def linear(x, weight, bias=None):
         if weight.dim() != 2:
             raise AccError(f"fp8.linear: weight [N, K] expected, got {tuple(weight.shape)}")
     N, K = weight.shape
-    if x.dim() < 1 or x.shape[-1] != K or N < 1 or K < 1:
+    if x.dim() < 1 or x.shape[-1] != K or not (1 <= N <= _MAX_DIM and 1 <= K <= _MAX_DIM):
         raise AccError(f"fp8.linear: x {tuple(x.shape)} and weight {(N, K)} do not match")
     if weight.device != x.device:
         raise AccError(f"fp8.linear: weight on {weight.device}, x on {x.device}")
@@ -162,23 +146,20 @@ def linear(x, weight, bias=None):
         x.requires_grad or (not frozen and weight.requires_grad)
         or (bias is not None and bias.requires_grad))
     x = x.contiguous()
-    wq = wt = None
+    wq = None
     if frozen:
         if not weight.square:
             raise AccError("fp8.linear: a frozen weight needs blocks of 128 x 128 "
                            "(quantize(w, square=True))")
-        wq = (weight.q, weight.s)
-        if weight.t is not None:
-            wt = (weight.t.q, weight.t.s)
-        elif grad and x.requires_grad:
+        if grad and x.requires_grad and weight.t is None:
             raise AccError("fp8.linear: the gradient of x needs the transposed weight "
                            "(quantize(w, square=True, transposed=True))")
-        weight = None
+        wq, weight = weight, None
     else:
         weight = weight.contiguous()
     if not grad:
         return _forward(x, weight, bias, wq, N)[0]
-    return _LinearFn.apply(x, weight, bias, wq, wt, N)
+    return _LinearFn.apply(x, weight, bias, wq, N)
 
 
 class Linear(nn.Linear):

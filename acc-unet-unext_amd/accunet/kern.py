@@ -663,15 +663,32 @@ def distill_bwd(z, save, up, reduction, held, dz, B, S, V, K, T, weight):
 
 
 # 8-bit linear layer
-def fp8_quantize(x, square, q, s, qt, st, sum_, R, C):
-    n = int(_lib.load().accunet_fp8_sum_ws_elems(R, C)) if sum_ is not None else 0
-    ws = workspace(n, x.device) if n else None
+def fp8_quantize(x, square, q, s, qt, st, R, C):
     _call_on((x,), "accunet_fp8_quantize", _a(x), 1 if square else 0, _a(q), _a(s), _a(qt), _a(st),
-             _a(sum_), _a(ws), n, R, C, _dt(x))
+             R, C, _dt(x))
 
 
-def fp8_gemm(a, sa, b, sb, bias, c, M, N, K):
-    n = int(_lib.load().accunet_fp8_gemm_ws_elems(M, N, K))
-    ws = workspace(n, a.device) if n else None
-    _call_on((a, b, bias), "accunet_fp8_gemm", _a(a), _a(sa), _a(b), _a(sb), _a(bias), _a(c),
-             _a(ws), n, M, N, K, _dt(c))
+def _bytes(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+def fp8_linear_fwd(x, w, wq, wqs, bias, y, need_w, need_wt, M, N, K):
+    """y; returns what a backward needs of x (need_w) and of an fp32 w (need_wt)."""
+    lib = _lib.load()
+    need_w, need_wt = 1 if need_w else 0, 1 if need_wt else 0
+    n = lib.accunet_fp8_linear_save_bytes(M, N, K, need_w, need_wt) if need_w or need_wt else 0
+    m = lib.accunet_fp8_linear_ws_bytes(M, N, K, 0 if w is None else 1)
+    save = _bytes(n, x.device) if n else None
+    ws = _bytes(m, x.device)
+    _call_on((x, w, wq, bias), "accunet_fp8_linear_fwd", _a(x), _a(w), _a(wq), _a(wqs), _a(bias),
+             _a(y), need_w, need_wt, _a(save), n, _a(ws), m, M, N, K, _dt(x))
+    return save
+
+
+def fp8_linear_bwd(dy, save, need_w, need_wt, wt, wts, dx, dw, db, M, N, K):
+    m = _lib.load().accunet_fp8_linear_bwd_ws_bytes(M, N, K, 0 if dx is None else 1,
+                                                    0 if dw is None else 1, 0 if db is None else 1)
+    ws = _bytes(m, dy.device)
+    _call_on((dy, save, wt), "accunet_fp8_linear_bwd", _a(dy), _a(save), 1 if need_w else 0,
+             1 if need_wt else 0, _a(wt), _a(wts), _a(dx), _a(dw), _a(db), _a(ws), m, M, N, K,
+             _dt(dy))

@@ -29,7 +29,7 @@ blocknorm_bwd_kernel(const BlockNormArgs a) {
   __shared__ float red[2][2][16];
   __shared__ float fold[WPR == 1 ? 4 : 1][2][WPR == 1 ? NE * 64 : 1];
   // sum g*A, sum g*B over the samples of the block; each thread owns its columns
-  __shared__ float tot[POST ? 2 : 1][POST ? NE * RT : 1];
+  __shared__ float tot[2][POST ? NE * RT : 1];
   int turn = 0;
   const int t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int sub = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;

@@ -37,5 +37,68 @@ ACC_DEV unsigned fp8_pack4(float a, float b, float c, float d) {
   return (unsigned)r;
 }
 
+typedef unsigned fp8_u4 __attribute__((ext_vector_type(4), aligned(2)));
+// n elements at p, zeros behind them; 16-byte loads, which the card takes at any address
+template <typename T>
+ACC_DEV void fp8_load8(const T* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    const fp8_u4 a = *reinterpret_cast<const fp8_u4*>(p);
+    if constexpr (sizeof(T) == 4) {
+      const fp8_u4 b = *reinterpret_cast<const fp8_u4*>(p + 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        v[u] = __uint_as_float(a[u]);
+        v[4 + u] = __uint_as_float(b[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        v[2 * u] = bflo(a[u]);
+        v[2 * u + 1] = bfhi(a[u]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = u < n ? ld1(p + u) : 0.f;
+  }
+}
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+// 8 e4m3 bytes as bf16, times a power of two
+ACC_DEV v8b fp8_widen(int lo, int hi, float scale) {
+  const v2b a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, false);
+  const v2b b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, true);
+  const v2b c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, false);
+  const v2b d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, true);
+  return (v8b){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 static inline long fp8_pad(long c) { return (c + 127) / 128 * 128; }
 static inline long fp8_scale_pitch(long c) { return ((c + 127) / 128 + 3) / 4 * 4; }
+
+// internal entry points (fp8_quant.hip, fp8_gemm.hip, fp8_token.hip)
+#define FP8_MAX_DIM (1L << 22)  // features: K, N
+static inline int fp8_check(long M, long K, long N, int dt) {
+  if (M <= 0 || K <= 0 || N <= 0 || K > FP8_MAX_DIM || N > FP8_MAX_DIM || M > (1L << 30))
+    return ACC_EBADSHAPE;
+  return dt == ACC_F32 || dt == ACC_BF16 ? ACC_OK : ACC_EBADARG;
+}
+// q, s and / or qt, st of x [R][C]; sum: column sums through ws (fp8_sum_elems fp32)
+size_t fp8_sum_elems(long R, int C);
+void fp8_quantize(const void* x, int dt, bool square, unsigned char* q, unsigned char* s,
+                  unsigned char* qt, unsigned char* st, float* sum, float* ws, long R, int C,
+                  hipStream_t str);
+// c [M][N] = A B^T (+ bias); ws: fp8_gemm_elems fp32
+size_t fp8_gemm_elems(long M, long N, long K);
+void fp8_gemm(const unsigned char* a, const unsigned char* sa, const unsigned char* b,
+              const unsigned char* sb, const float* bias, void* c, int cdt, float* ws, long M,
+              long N, long K, hipStream_t st);
+// up to 16 tokens: x is quantised where it is used
+#define FP8_TOKENS 16
+void fp8_token(const void* x, const unsigned char* w, const unsigned char* sw, const float* bias,
+               void* y, int dt, int M, int N, int K, hipStream_t st);

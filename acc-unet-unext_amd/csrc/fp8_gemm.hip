@@ -18,21 +18,6 @@
 // yield is not stored.
 #include "fp8.h"
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-
-// 8 e4m3 bytes as bf16, times a power of two
-ACC_DEV v8b fp8_widen(int lo, int hi, float scale) {
-  const v2b a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, false);
-  const v2b b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, true);
-  const v2b c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, false);
-  const v2b d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, true);
-  return (v8b){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
 // Lane i copies 16 (4) bytes from its `src` to lds + 16 i (4 i), lds the same for the wave.
 // From inline asm: the compiler would otherwise wait for every copy before any LDS read of
 // the array. The wave waits for its copies itself, before the barrier that publishes them.
@@ -256,35 +241,27 @@ static int fp8_splits(long M, long N, long K) {
   return (int)((quads + per - 1) / per);
 }
 
-extern "C" size_t accunet_fp8_gemm_ws_elems(long M, long N, long K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+size_t fp8_gemm_elems(long M, long N, long K) {
   const int s = fp8_splits(M, N, K);
   return s > 1 ? (size_t)s * M * N : 0;
 }
 
-extern "C" int accunet_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb,
-                                const float* bias, void* c, float* ws, size_t ws_elems, long M,
-                                long N, long K, int cdt, void* stream) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > (1L << 30)) return ACC_EBADSHAPE;
+void fp8_gemm(const unsigned char* a, const unsigned char* sa, const unsigned char* b,
+              const unsigned char* sb, const float* bias, void* c, int cdt, float* ws, long M,
+              long N, long K, hipStream_t st) {
   // 256 x 256 tiles where they alone give every CU one, 128 x 128 else
   const bool big = ((M + 255) / 256) * ((N + 255) / 256) >= 256;
   const int bt = big ? 256 : 128;
   const long tm = (M + bt - 1) / bt, tn = (N + bt - 1) / bt;
-  if (tn > 0x7fffffffL || tm * tn > 0x7ffffff0L) return ACC_EBADSHAPE;
-  if (!a || !sa || !b || !sb || !c) return ACC_EBADARG;
-  if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)sa | (uintptr_t)sb) & 3) return ACC_EBADARG;
-  if (ws_elems < accunet_fp8_gemm_ws_elems(M, N, K)) return ACC_EBADARG;
   Fp8GemmArgs g;
-  g.a = (const unsigned char*)a; g.sa = (const unsigned char*)sa;
-  g.b = (const unsigned char*)b; g.sb = (const unsigned char*)sb;
+  g.a = a; g.sa = sa; g.b = b; g.sb = sb;
   g.c = c; g.bias = bias; g.slab = ws;
   g.M = M; g.N = N; g.KP = (int)fp8_pad(K); g.SP = (int)fp8_scale_pitch(K);
   g.tiles_m = (int)tm; g.tiles_n = (int)tn;
   const int splits = fp8_splits(M, N, K);
   const int quads = (g.KP / 128 + 3) / 4;
   g.kt_per = (quads + splits - 1) / splits * 4;
-  hipStream_t st = (hipStream_t)stream;
-  const int rc = with_dt(cdt, [&](auto tag) {
+  with_dt(cdt, [&](auto tag) {
     using T = decltype(tag);
     constexpr bool WIDE = sizeof(T) == 4;
     const dim3 grid((unsigned)((tm * tn + 7) / 8 * 8), 1, splits);
@@ -293,14 +270,12 @@ extern "C" int accunet_fp8_gemm(const void* a, const void* sa, const void* b, co
       hipLaunchKernelGGL((fp8_gemm_kernel<T, true, WIDE, 2, 2, 4, 4>), grid, dim3(256), 0, st, g);
       hipLaunchKernelGGL(fp8_join_kernel<T>, dim3((unsigned)((M * N + 255) / 256)), dim3(256), 0,
                          st, ws, splits, bias, (T*)c, M * N, N);
-    } else {
-      g.vec = N % 4 == 0 && ((uintptr_t)c & (4 * sizeof(T) - 1)) == 0;
-      if (big)
-        hipLaunchKernelGGL((fp8_gemm_kernel<T, false, WIDE, 2, 4, 8, 4>), grid, dim3(512), 0, st, g);
-      else
-        hipLaunchKernelGGL((fp8_gemm_kernel<T, false, WIDE, 2, 2, 4, 4>), grid, dim3(256), 0, st, g);
+      return;
     }
+    g.vec = N % 4 == 0 && ((uintptr_t)c & (4 * sizeof(T) - 1)) == 0;
+    if (big)
+      hipLaunchKernelGGL((fp8_gemm_kernel<T, false, WIDE, 2, 4, 8, 4>), grid, dim3(512), 0, st, g);
+    else
+      hipLaunchKernelGGL((fp8_gemm_kernel<T, false, WIDE, 2, 2, 4, 4>), grid, dim3(256), 0, st, g);
   });
-  if (rc != ACC_OK) return rc;
-  return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
 }

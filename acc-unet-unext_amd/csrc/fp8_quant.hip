@@ -3,24 +3,12 @@
 // element is written for each form.
 #include "fp8.h"
 
-template <typename T>
-ACC_DEV void fp8_load8(const T* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    const float4 a = ldq(p), b = ldq(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = u < n ? ld1(p + u) : 0.f;
-  }
-}
-
 // Rows only: 16 threads a block of 128, 8 elements each. A thread past the scale pitch's
 // last block leaves; one in the padding writes the padding.
 template <typename T>
 __global__ void __launch_bounds__(256)
 fp8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
-                unsigned char* __restrict__ s, long R, int C, int CP, int SP, int vec) {
+                unsigned char* __restrict__ s, long R, int C, int CP, int SP) {
   const int per = SP * 16;  // threads a row
   const long g = blockIdx.x * 256L + threadIdx.x;
   const long row = g / per;
@@ -28,7 +16,7 @@ fp8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   const int t = (int)(g - row * per);
   const int c = t * 8;
   float v[8];
-  fp8_load8(x + row * C + c, C - c, vec, v);
+  fp8_load8(x + row * C + c, C - c, v);
   unsigned m = 0u;
 #pragma unroll
   for (int u = 0; u < 8; ++u) m = max(m, fp8_finite_bits(v[u]));
@@ -45,19 +33,19 @@ fp8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   if ((t & 15) == 0) s[row * SP + (t >> 4)] = (unsigned char)e;
 }
 
-// A 128 x 128 tile: thread t holds columns 8 (t % 16) .. + 7 of rows t / 16 + 16 i.
+// A 128 x 128 tile: thread t holds columns 8 (t % 16) .. + 7 of rows 8 (t / 16) .. + 7.
 //   q, s     blocks 1 x 128 along the rows          (square: the tile is one block)
 //   qt, st   the transposed matrix [C][RP], blocks 1 x 128 along the rows of x
 //   sum      [tiles of rows][C] column sums
-// The transposed bytes go through LDS: [column][row], a column's 128 bytes padded to 132 so
-// that the 16 columns a wave writes at once lie in different banks.
+// The transposed bytes go through LDS: [column][row], the 8 rows of a column as two dwords; a
+// column's 128 bytes are padded to 132, which spreads a wave's dwords evenly over the banks.
 #define FP8_TP 132
 template <typename T>
 __global__ void __launch_bounds__(256)
 fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
                 unsigned char* __restrict__ s, unsigned char* __restrict__ qt,
                 unsigned char* __restrict__ st, float* __restrict__ sum, long R, int C, int CP,
-                int SP, long RP, int SPT, int square, int vec) {
+                int SP, long RP, int SPT, int square) {
   __shared__ __attribute__((aligned(16))) unsigned char tile[128 * FP8_TP];
   __shared__ unsigned cmax[16][128];
   __shared__ unsigned wmax[4];
@@ -69,8 +57,8 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   float v[8][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const long r = r0 + rg + 16 * i;
-    fp8_load8(x + r * C + c, r < R ? C - c : 0, vec, v[i]);
+    const long r = r0 + rg * 8 + i;
+    fp8_load8(x + r * C + c, r < R ? C - c : 0, v[i]);
   }
   int e[8];
   unsigned all = 0u;
@@ -96,7 +84,7 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   if (q) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const long r = r0 + rg + 16 * i;
+      const long r = r0 + rg * 8 + i;
       if (r >= R) continue;
       const float inv = fp8_inverse(e[i]);
       uint2 w;
@@ -135,13 +123,13 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
 #pragma unroll
       for (int u = 0; u < 8; ++u) inv[u] = fp8_inverse(cb[cg * 8 + u]);
     }
-    // rows rg + 16 i of this thread: byte (column, row)
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        tile[(cg * 8 + u) * FP8_TP + rg + 16 * i] =
-            (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(v[i][u] * inv[u], 0.f, 0, false);
+    for (int u = 0; u < 8; ++u) {
+      const float iv = inv[u];
+      unsigned* dst = reinterpret_cast<unsigned*>(tile + (cg * 8 + u) * FP8_TP + rg * 8);
+      dst[0] = fp8_pack4(v[0][u] * iv, v[1][u] * iv, v[2][u] * iv, v[3][u] * iv);
+      dst[1] = fp8_pack4(v[4][u] * iv, v[5][u] * iv, v[6][u] * iv, v[7][u] * iv);
+    }
     __syncthreads();
     // 8 threads a column, 16 bytes each
     for (int k = t; k < 128 * 8; k += 256) {
@@ -191,39 +179,37 @@ fp8_colsum_kernel(const float* __restrict__ part, long n, int C, float* __restri
   if (g == 0 && c < C) out[c] = (float)(((red[0][cl] + red[1][cl]) + red[2][cl]) + red[3][cl]);
 }
 
-extern "C" size_t accunet_fp8_sum_ws_elems(long R, int C) {
-  return R > 0 && C > 0 ? (size_t)((R + 127) / 128) * C : 0;
-}
+size_t fp8_sum_elems(long R, int C) { return (size_t)((R + 127) / 128) * C; }
 
-extern "C" int accunet_fp8_quantize(const void* x, int square, void* q, void* s, void* qt, void* st,
-                                    float* sum, float* ws, size_t ws_elems, long R, int C, int dt,
-                                    void* stream) {
-  if (R <= 0 || C <= 0 || (R + 127) / 128 > 0x7fffffffL || C > 65535 * 128) return ACC_EBADSHAPE;
-  if (!x || (q != nullptr) != (s != nullptr) || (qt != nullptr) != (st != nullptr) ||
-      (!q && !qt))
-    return ACC_EBADARG;
-  if (sum && (!ws || ws_elems < accunet_fp8_sum_ws_elems(R, C))) return ACC_EBADARG;
+void fp8_quantize(const void* x, int dt, bool square, unsigned char* q, unsigned char* s,
+                  unsigned char* qt, unsigned char* st, float* sum, float* ws, long R, int C,
+                  hipStream_t str) {
   const int CP = (int)fp8_pad(C), SP = (int)fp8_scale_pitch(C);
   const long RP = fp8_pad(R);
   const int SPT = (int)fp8_scale_pitch(R);
-  hipStream_t str = (hipStream_t)stream;
-  const int rc = with_dt(dt, [&](auto tag) {
+  with_dt(dt, [&](auto tag) {
     using T = decltype(tag);
-    // 16-byte loads of 4 (fp32) or 8-byte loads of 4 (bf16)
-    const int vec = C % 4 == 0 && ((uintptr_t)x & (4 * sizeof(T) - 1)) == 0;
     if (!square && !qt && !sum) {
       const long n = R * SP * 16;
       hipLaunchKernelGGL(fp8_rows_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, str,
-                         (const T*)x, (unsigned char*)q, (unsigned char*)s, R, C, CP, SP, vec);
+                         (const T*)x, q, s, R, C, CP, SP);
       return;
     }
     hipLaunchKernelGGL(fp8_tile_kernel<T>, dim3((unsigned)(RP / 128), CP / 128), dim3(256), 0, str,
-                       (const T*)x, (unsigned char*)q, (unsigned char*)s, (unsigned char*)qt,
-                       (unsigned char*)st, sum ? ws : nullptr, R, C, CP, SP, RP, SPT, square, vec);
+                       (const T*)x, q, s, qt, st, sum ? ws : nullptr, R, C, CP, SP, RP, SPT,
+                       square ? 1 : 0);
     if (sum)
       hipLaunchKernelGGL(fp8_colsum_kernel, dim3(ceil_div(C, 64)), dim3(256), 0, str, ws, RP / 128,
                          C, sum);
   });
+}
+
+extern "C" int accunet_fp8_quantize(const void* x, int square, void* q, void* s, void* qt, void* st,
+                                    long R, int C, int dt, void* stream) {
+  const int rc = fp8_check(R, C, 1, dt);
   if (rc != ACC_OK) return rc;
+  if (!x || !q || !s || (qt != nullptr) != (st != nullptr)) return ACC_EBADARG;
+  fp8_quantize(x, dt, square != 0, (unsigned char*)q, (unsigned char*)s, (unsigned char*)qt,
+               (unsigned char*)st, nullptr, nullptr, R, C, (hipStream_t)stream);
   return hipGetLastError() == hipSuccess ? ACC_OK : ACC_ELAUNCH;
 }

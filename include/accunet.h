@@ -550,21 +550,30 @@ int accunet_distill_bwd(const void* z, void* save, size_t save_bytes, const floa
  * [128 j, 128 j + 128), SP = CP / 128 rounded up to 4 (padding 127). e is the least integer
  * with amax <= 448 * 2^e over the block's finite elements, in [-126, 120]; 0 for zeros.
  *   accunet_fp8_quantize: x [R][C] of storage dt -> q, s with blocks 1 x 128 (128 x 128
- *     with square, the byte repeated over the rows), and / or qt, st: the transposed matrix
- *     [C][R] with blocks along R (square: the same blocks). sum (fp32 [C], or NULL): the
- *     column sums of x, through ws of accunet_fp8_sum_ws_elems fp32 elements.
- *   accunet_fp8_gemm: c [M][N] (storage cdt) = A B^T (+ bias fp32 [N]) of quantised A [M][K]
- *     and B [N][K], fp32 accumulation; ws: accunet_fp8_gemm_ws_elems fp32 elements.
- * q, qt: 16-byte aligned; s, st: 4-byte aligned.
+ *     with square, the byte repeated over the rows); qt, st (or NULL): the transposed matrix
+ *     [C][R] with blocks along R (square: the same blocks).
+ *   accunet_fp8_linear_fwd: y [M][N] (storage dt, as x [M][K]) = Q(x) Q(w)^T (+ bias fp32 [N]);
+ *     the weight as fp32 w [N][K], or quantised in squares (wq, wqs). For a backward, save
+ *     (accunet_fp8_linear_save_bytes) keeps the transposed x (need_w) and the transposed
+ *     weight (need_wt, with w).
+ *   accunet_fp8_linear_bwd: dx [M][K] (storage dt), dw fp32 [N][K], db fp32 [N], each or NULL,
+ *     from dy [M][N]; need_w, need_wt as in the forward; wt, wts: the transposed quantised
+ *     weight where save does not hold it.
+ *   ws: accunet_fp8_linear_ws_bytes / _bwd_ws_bytes bytes. fp32 accumulation.
+ * q, qt: 16-byte aligned; s, st: 4-byte; save, ws: 256-byte. K, N <= 2^22.
  * ------------------------------------------------------------------------- */
-size_t accunet_fp8_sum_ws_elems(long R, int C);
-int accunet_fp8_quantize(const void* x, int square, void* q, void* s, void* qt, void* st,
-                         float* sum, float* ws, size_t ws_elems, long R, int C, int dt,
-                         void* stream);
-size_t accunet_fp8_gemm_ws_elems(long M, long N, long K);
-int accunet_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb,
-                     const float* bias, void* c, float* ws, size_t ws_elems, long M, long N, long K,
-                     int cdt, void* stream);
+int accunet_fp8_quantize(const void* x, int square, void* q, void* s, void* qt, void* st, long R,
+                         int C, int dt, void* stream);
+size_t accunet_fp8_linear_save_bytes(long M, long N, long K, int need_w, int need_wt);
+size_t accunet_fp8_linear_ws_bytes(long M, long N, long K, int own_w);
+size_t accunet_fp8_linear_bwd_ws_bytes(long M, long N, long K, int dx, int dw, int db);
+int accunet_fp8_linear_fwd(const void* x, const float* w, const void* wq, const void* wqs,
+                           const float* bias, void* y, int need_w, int need_wt, void* save,
+                           size_t save_bytes, void* ws, size_t ws_bytes, long M, long N, long K,
+                           int dt, void* stream);
+int accunet_fp8_linear_bwd(const void* dy, const void* save, int need_w, int need_wt,
+                           const void* wt, const void* wts, void* dx, float* dw, float* db,
+                           void* ws, size_t ws_bytes, long M, long N, long K, int dt, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from accunet import _lib
+from accunet import _lib, kern
 
 U = 2.0 ** -24
 
@@ -32,18 +32,30 @@ def test_refusals_on_the_host():
     lib = _lib.load()
     ok = 16
     q = lib.accunet_fp8_quantize
-    assert q(ok, 0, ok, ok, None, None, None, None, 0, 0, 8, 0, None) == -1
-    assert q(ok, 0, ok, None, None, None, None, None, 0, 2, 8, 0, None) == -2   # q without s
-    assert q(ok, 0, None, None, None, None, None, None, 0, 2, 8, 0, None) == -2  # nothing to make
-    assert q(ok, 0, ok, ok, None, None, ok, ok, 7, 2, 8, 0, None) == -2         # sums: workspace
-    assert q(ok, 0, ok, ok, None, None, None, None, 0, 2, 8, 3, None) == -2     # storage type
-    assert lib.accunet_fp8_sum_ws_elems(129, 8) == 16
-    g = lib.accunet_fp8_gemm
-    assert g(ok, ok, ok, ok, None, ok, None, 0, 0, 8, 8, 0, None) == -1
-    assert g(ok, ok, None, ok, None, ok, None, 0, 8, 8, 8, 0, None) == -2
-    assert g(8, ok, ok, ok, None, ok, None, 0, 8, 8, 8, 0, None) == -2           # alignment
-    n = lib.accunet_fp8_gemm_ws_elems(8, 8, 4096)
-    assert n > 0 and g(ok, ok, ok, ok, None, ok, ok, n - 1, 8, 8, 4096, 0, None) == -2
+    assert q(ok, 0, ok, ok, None, None, 0, 8, 0, None) == -1
+    assert q(ok, 0, ok, None, None, None, 2, 8, 0, None) == -2   # q without s
+    assert q(ok, 0, ok, ok, ok, None, 2, 8, 0, None) == -2       # qt without st
+    assert q(ok, 0, ok, ok, None, None, 2, 8, 3, None) == -2     # storage type
+    assert q(ok, 0, ok, ok, None, None, 2, (1 << 22) + 1, 0, None) == -1
+    fwd, bwd, al = lib.accunet_fp8_linear_fwd, lib.accunet_fp8_linear_bwd, 256
+    n = lib.accunet_fp8_linear_ws_bytes(8, 8, 4096, 1)
+    k = lib.accunet_fp8_linear_save_bytes(8, 8, 4096, 1, 1)
+    assert n > 0 and k > 0 and lib.accunet_fp8_linear_ws_bytes(0, 8, 8, 1) == 0
+
+    def f_(x=ok, w=ok, wq=None, wqs=None, need_w=1, need_wt=1, save=al, kb=k, ws=al, nb=n, M=8, dt=0):
+        return fwd(x, w, wq, wqs, None, ok, need_w, need_wt, save, kb, ws, nb, M, 8, 4096, dt, None)
+
+    assert f_(M=0) == -1 and f_(dt=2) == -2 and f_(x=None) == -2 and f_(nb=n - 1) == -2
+    assert f_(kb=k - 1) == -2 and f_(save=None) == -2 and f_(ws=16) == -2 and f_(wq=ok) == -2
+    assert f_(w=None) == -2 and f_(w=None, wq=ok, wqs=ok) == -2  # need_wt without w
+    assert f_(w=None, wq=8, wqs=ok, need_wt=0) == -2             # alignment
+    m = lib.accunet_fp8_linear_bwd_ws_bytes(8, 8, 4096, 1, 1, 1)
+
+    def b_(dy=ok, save=al, need_w=1, need_wt=1, dx=ok, dw=ok, db=ok, mb=m):
+        return bwd(dy, save, need_w, need_wt, None, None, dx, dw, db, al, mb, 8, 8, 4096, 0, None)
+
+    assert b_(dy=None) == -2 and b_(mb=m - 1) == -2 and b_(save=None) == -2
+    assert b_(dx=None, dw=None, db=None) == -2 and b_(need_w=0) == -2 and b_(need_wt=0) == -2
 
 
 # ----------------------------------------------------------------------- the reference
@@ -113,14 +125,12 @@ def test_quantize(R, C, dtype):
     b = fp8.quantize(x, square=True, transposed=True)
     _assert_blocks(b, x, 128)
     assert torch.equal(b.values().t().contiguous(), b.t.values())
-    # the transposed form with blocks along the rows, and the column sums
-    s = torch.empty(C, device="cuda")
-    (q, sc), (qt, st) = fp8._quantize(x, R, C, cols=True, colsum=s)
+    # the transposed form with blocks along the rows
+    qt, st = fp8._new(C, R, x.device)
+    q, sc = fp8._new(R, C, x.device)
+    kern.fp8_quantize(x, False, q, sc, qt, st, R, C)
     _assert_blocks(fp8.Fp8Blocks(q, sc, R, C, False), x, 1)
     _assert_blocks(fp8.Fp8Blocks(qt, st, C, R, False), x.t().contiguous(), 1)
-    want = x.double().sum(0).cpu()
-    mag = x.double().abs().sum(0).cpu()
-    assert bool(((s.double().cpu() - want).abs() <= 32 * U * mag).all())
 
 
 @pytest.mark.gpu
@@ -169,7 +179,7 @@ def _product_ok(got, a, b, bias=None, n=None):
     assert float(over.max()) <= 0, float(over.max())
 
 
-GEMMS = [(1, 1, 1), (1, 300, 513), (5, 17, 128), (17, 129, 1000), (64, 96, 2049), (128, 128, 512),
+GEMMS = [(1, 1, 1), (16, 40, 1100), (9, 250, 9000), (3000, 5700, 300), (1, 4096, 96), (1, 300, 513), (5, 17, 128), (17, 129, 1000), (64, 96, 2049), (128, 128, 512),
          (130, 250, 640), (333, 777, 160), (2, 640, 4100), (1000, 131, 257), (129, 1500, 96),
          (2500, 1400, 130)]
 
@@ -194,12 +204,33 @@ def test_linear_forward_and_gradients(M, N, K, dtype):
     _product_ok(dw, _grid(dyc.t().contiguous())[0], _grid(xc.t().contiguous())[0])
     want, mag = dyc.double().sum(0), dyc.double().abs().sum(0)
     assert bool(((db.double().cpu() - want).abs() <= 32 * U * mag).all())
-    # a frozen weight gives the same bits
+    # a frozen weight stands for the same values; up to 16 tokens run another kernel then,
+    # whose sums have another order
     f = fp8.quantize(w, square=True, transposed=True)
     y2 = fp8.linear(x, f, b)
-    assert torch.equal(y, y2) and torch.equal(dx, torch.autograd.grad(y2, x, dy)[0])
+    _product_ok(y2, _grid(xc)[0], wg, b.detach().cpu())
+    assert torch.equal(dx, torch.autograd.grad(y2, x, dy)[0])
+    if M > 16:
+        assert torch.equal(y, y2)
     with torch.no_grad():
-        assert torch.equal(y, fp8.linear(x, fp8.quantize(w, square=True), b))
+        assert torch.equal(y2, fp8.linear(x, fp8.quantize(w, square=True), b))
+        assert torch.equal(y2, fp8.linear(x, w, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [2, 15, 16])
+def test_few_tokens(M, dtype):
+    """The kernel that quantises its tokens itself: ragged features, special values."""
+    fp8 = _mod()
+    x, w = _data(M, 333, dtype, 5), _data(45, 333, torch.float32, 6)
+    x[0, 130:260] = 0.0
+    wq = fp8.quantize(w.cuda(), square=True)
+    b = _data(1, 45, torch.float32, 7)[0]
+    _product_ok(fp8.linear(x.cuda(), wq, b.cuda()), _grid(x)[0], _grid(w, 128)[0], b)
+    x[1, 332] = math.nan
+    y = fp8.linear(x.cuda(), wq).cpu()
+    assert bool(torch.isnan(y[1]).all()) and bool(torch.isfinite(y[0]).all())
 
 
 @pytest.mark.gpu
