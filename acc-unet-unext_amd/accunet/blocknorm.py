@@ -35,8 +35,10 @@ def _forward(x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L, keep):
 
 def _apply(*args):
     """The formulas on checked arguments; the autograd node only where a gradient may flow."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
-        return _BlockNormFn.apply(*args)
+    if torch.is_grad_enabled():
+        for t in args[:8]:
+            if t is not None and t.requires_grad:
+                return _BlockNormFn.apply(*args)
     return _forward(*args, False)[:2]
 
 
@@ -72,14 +74,14 @@ class _BlockNormFn(torch.autograd.Function):
 def _param(t, C, name, x):
     if t is None:
         return None
-    if t.dtype != torch.float32 or tuple(t.shape) != (C,) or t.device != x.device:
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != C or t.get_device() != x.get_device():
         raise AccError(f"{name}: float32 [{C}] on {x.device} expected, got {t.dtype} "
                        f"{tuple(t.shape)} on {t.device}")
     return t.contiguous()
 
 
 def _act(t, name, x):
-    if t.dtype != x.dtype or t.device != x.device:
+    if t.dtype != x.dtype or t.get_device() != x.get_device():
         raise AccError(f"{name}: {x.dtype} on {x.device} expected, got {t.dtype} on {t.device}")
     return t.contiguous()
 
@@ -117,12 +119,10 @@ def sandwich_norm(x, f, post_weight=None, post_bias=None, scale=None, gate=None,
             raise AccError(f"sandwich_norm: gate {tuple(gate.shape)} is neither x's shape "
                            f"{tuple(x.shape)} nor one row per sample {shared}")
         gate = _act(gate, "sandwich_norm gate", x)
-    args = [_param(t, C, n, x) for t, n in
-            ((post_weight, "post_weight"), (post_bias, "post_bias"), (scale, "scale"),
-             (pre_weight, "pre_weight"), (pre_bias, "pre_bias"))]
-    f = _act(f, "sandwich_norm f", x)
-    return _apply(x.contiguous(), f, args[0], args[1], args[2], gate, args[3], args[4],
-                  kind == "layer", float(eps), bool(pre), L)
+    return _apply(x.contiguous(), _act(f, "sandwich_norm f", x),
+                  _param(post_weight, C, "post_weight", x), _param(post_bias, C, "post_bias", x),
+                  _param(scale, C, "scale", x), gate, _param(pre_weight, C, "pre_weight", x),
+                  _param(pre_bias, C, "pre_bias", x), kind == "layer", float(eps), bool(pre), L)
 
 
 def norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):

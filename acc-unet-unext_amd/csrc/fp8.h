@@ -38,29 +38,34 @@ ACC_DEV unsigned fp8_pack4(float a, float b, float c, float d) {
 }
 
 typedef unsigned fp8_u4 __attribute__((ext_vector_type(4), aligned(2)));
+// 8 neighbouring elements as loaded
+template <typename T>
+struct Fp8Raw {
+  fp8_u4 w[sizeof(T) / 2];
+  ACC_DEV float get(int u) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[u >> 2][u & 3]);
+    else return u & 1 ? bfhi(w[0][u >> 1]) : bflo(w[0][u >> 1]);
+  }
+};
 // n elements at p, zeros behind them; 16-byte loads, which the card takes at any address
 template <typename T>
-ACC_DEV void fp8_load8(const T* p, int n, float (&v)[8]) {
+ACC_DEV Fp8Raw<T> fp8_load8(const T* p, int n) {
+  Fp8Raw<T> r;
   if (n >= 8) {
-    const fp8_u4 a = *reinterpret_cast<const fp8_u4*>(p);
-    if constexpr (sizeof(T) == 4) {
-      const fp8_u4 b = *reinterpret_cast<const fp8_u4*>(p + 4);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        v[u] = __uint_as_float(a[u]);
-        v[4 + u] = __uint_as_float(b[u]);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        v[2 * u] = bflo(a[u]);
-        v[2 * u + 1] = bfhi(a[u]);
-      }
-    }
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+      r.w[k] = *reinterpret_cast<const fp8_u4*>(p + 4 * k * (4 / sizeof(T)));
   } else {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = u < n ? ld1(p + u) : 0.f;
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) r.w[k] = (fp8_u4){0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (u < n) {
+        if constexpr (sizeof(T) == 4) r.w[u >> 2][u & 3] = __float_as_uint(p[u]);
+        else r.w[0][u >> 1] |= (unsigned)p[u] << (16 * (u & 1));
+      }
   }
+  return r;
 }
 
 typedef int v8i __attribute__((ext_vector_type(8)));

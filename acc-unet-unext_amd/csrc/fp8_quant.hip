@@ -15,11 +15,14 @@ fp8_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   if (row >= R) return;
   const int t = (int)(g - row * per);
   const int c = t * 8;
+  const Fp8Raw<T> raw = fp8_load8(x + row * C + c, C - c);
   float v[8];
-  fp8_load8(x + row * C + c, C - c, v);
   unsigned m = 0u;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) m = max(m, fp8_finite_bits(v[u]));
+  for (int u = 0; u < 8; ++u) {
+    v[u] = raw.get(u);
+    m = max(m, fp8_finite_bits(v[u]));
+  }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
   const int e = fp8_scale_byte(m);
@@ -54,11 +57,12 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4;
   const long r0 = (long)blockIdx.x * 128;
   const int c0 = blockIdx.y * 128, c = c0 + cg * 8;
-  float v[8][8];
+  // kept as loaded: 32 registers for bf16, and twice the blocks a CU
+  Fp8Raw<T> raw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const long r = r0 + rg * 8 + i;
-    fp8_load8(x + r * C + c, r < R ? C - c : 0, v[i]);
+    raw[i] = fp8_load8(x + r * C + c, r < R ? C - c : 0);
   }
   int e[8];
   unsigned all = 0u;
@@ -66,7 +70,7 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
   for (int i = 0; i < 8; ++i) {
     unsigned m = 0u;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) m = max(m, fp8_finite_bits(v[i][u]));
+    for (int u = 0; u < 8; ++u) m = max(m, fp8_finite_bits(raw[i].get(u)));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
     e[i] = fp8_scale_byte(m);
@@ -88,8 +92,8 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
       if (r >= R) continue;
       const float inv = fp8_inverse(e[i]);
       uint2 w;
-      w.x = fp8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-      w.y = fp8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+      w.x = fp8_pack4(raw[i].get(0) * inv, raw[i].get(1) * inv, raw[i].get(2) * inv, raw[i].get(3) * inv);
+      w.y = fp8_pack4(raw[i].get(4) * inv, raw[i].get(5) * inv, raw[i].get(6) * inv, raw[i].get(7) * inv);
       *reinterpret_cast<uint2*>(q + r * CP + c) = w;
       if (cg == 0) s[r * SP + blockIdx.y] = (unsigned char)e[i];
       // the scale row's padding, written once
@@ -109,7 +113,7 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
       for (int u = 0; u < 8; ++u) {
         unsigned m = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, fp8_finite_bits(v[i][u]));
+        for (int i = 0; i < 8; ++i) m = max(m, fp8_finite_bits(raw[i].get(u)));
         cmax[rg][cg * 8 + u] = m;
       }
       __syncthreads();
@@ -127,8 +131,8 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
     for (int u = 0; u < 8; ++u) {
       const float iv = inv[u];
       unsigned* dst = reinterpret_cast<unsigned*>(tile + (cg * 8 + u) * FP8_TP + rg * 8);
-      dst[0] = fp8_pack4(v[0][u] * iv, v[1][u] * iv, v[2][u] * iv, v[3][u] * iv);
-      dst[1] = fp8_pack4(v[4][u] * iv, v[5][u] * iv, v[6][u] * iv, v[7][u] * iv);
+      dst[0] = fp8_pack4(raw[0].get(u) * iv, raw[1].get(u) * iv, raw[2].get(u) * iv, raw[3].get(u) * iv);
+      dst[1] = fp8_pack4(raw[4].get(u) * iv, raw[5].get(u) * iv, raw[6].get(u) * iv, raw[7].get(u) * iv);
     }
     __syncthreads();
     // 8 threads a column, 16 bytes each
@@ -152,7 +156,7 @@ fp8_tile_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
     for (int u = 0; u < 8; ++u) {
       float a = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a += v[i][u];
+      for (int i = 0; i < 8; ++i) a += raw[i].get(u);
       csum[rg][cg * 8 + u] = a;
     }
     __syncthreads();

@@ -10,13 +10,13 @@
 #include "fp8.h"
 
 #define FP8_TW 8  // waves a block
-#define FP8_TU 4  // k-tiles whose weights a wave has in flight
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(64 * FP8_TW)
 fp8_token_kernel(const T* __restrict__ x, const unsigned char* __restrict__ w,
                  const unsigned char* __restrict__ sw, const float* __restrict__ bias,
                  T* __restrict__ y, int M, int N, int K, int KP, int SP) {
+  constexpr int FP8_TU = sizeof(T) == 4 ? 2 : 4;  // k-tiles a wave has in flight
   __shared__ float4 red[FP8_TW][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l15 = lane & 15, kg = lane >> 4;
@@ -29,6 +29,7 @@ fp8_token_kernel(const T* __restrict__ x, const unsigned char* __restrict__ w,
   for (int k0 = wave; k0 < tiles; k0 += FP8_TW * FP8_TU) {
     v8i fw[FP8_TU];
     int bw[FP8_TU];
+    Fp8Raw<T> rx[FP8_TU][4];
 #pragma unroll
     for (int u = 0; u < FP8_TU; ++u) {
       const int kt = min(k0 + u * FP8_TW, tiles - 1);
@@ -36,20 +37,23 @@ fp8_token_kernel(const T* __restrict__ x, const unsigned char* __restrict__ w,
       const v4i hi = *reinterpret_cast<const v4i*>(wr + (long)kt * 128 + 16);
       fw[u] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       bw[u] = sr[kt];
+      const int left = l15 < M ? K - (kt * 128 + kg * 32) : 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rx[u][q] = fp8_load8(xr + kt * 128 + q * 8, left - q * 8);
     }
 #pragma unroll
     for (int u = 0; u < FP8_TU; ++u) {
       const int kt = k0 + u * FP8_TW;
       if (kt >= tiles) break;  // the same for the wave
-      const int left = l15 < M ? K - (kt * 128 + kg * 32) : 0;
       float v[4][8];
       unsigned m = 0u;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        fp8_load8(xr + kt * 128 + q * 8, left - q * 8, v[q]);
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, fp8_finite_bits(v[q][e]));
-      }
+        for (int e = 0; e < 8; ++e) {
+          v[q][e] = rx[u][q].get(e);
+          m = max(m, fp8_finite_bits(v[q][e]));
+        }
       m = max(m, (unsigned)__shfl_xor((int)m, 16));
       m = max(m, (unsigned)__shfl_xor((int)m, 32));
       const int b = fp8_scale_byte(m);

@@ -162,14 +162,16 @@ def test_quantize_values_at_the_edges():
     _assert_blocks(fp8.quantize(x.cuda(), square=True), x.cuda(), 128)
 
 
-def _product_ok(got, a, b, bias=None, n=None):
+def _product_ok(got, a, b, bias=None):
+    a, b = a.cuda(), b.cuda()  # fp64 products of fp64 values
+    bias = bias.cuda() if bias is not None else None
     want = a @ b.t()
     mag = a.abs() @ b.abs().t()
     if bias is not None:
         want, mag = want + bias.double(), mag + bias.double().abs()
     K = a.shape[1]
     tol = (128 + K / 32 + 2) * U * mag
-    got = got.detach().cpu()
+    got = got.detach().cuda()
     assert got.shape == want.shape
     if got.dtype == torch.bfloat16:
         top = [torch.nn.functional.pad(t.abs(), (0, -K % 8)).view(t.shape[0], -1, 8).amax(2)
