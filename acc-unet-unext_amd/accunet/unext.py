@@ -20,6 +20,10 @@ Operator mapping (all compute in libaccunet_hip.so):
   GELU                         accunet_gelu_fwd/bwd
   relu(interpolate x2) + skip  accunet_up2_relu_add_fwd / accunet_up2_relu_bwd
   final 1x1 + sigmoid          ops.head
+Two options of the tokenised stages, off by default (the reference's network and its
+state_dict): UNext(linear="fp8") runs fc1 / fc2 in 8 bits (accunet.fp8, same parameters);
+UNext(sandwich=True) adds a norm and a residual scale after each block, fused with the
+residual add and the norm that follows it (accunet.blocknorm).
 Initial weights use PyTorch's default layer init (the reference's timm
 trunc_normal_ init, :52-64, is not reproduced: timm is not part of this image);
 load a reference state_dict for identical weights.
@@ -29,8 +33,9 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import kern, ops
+from . import fp8, kern, ops
 from ._lib import ACT_NONE
+from .blocknorm import sandwich_norm
 
 
 def _empty(shape, like, dtype=torch.float32):
@@ -192,8 +197,12 @@ class DWConv(nn.Module):
 class shiftmlp(nn.Module):  # noqa: N801 (reference name)
     """UNext.py:38-118 (shift_size 5, GELU, no dropout at drop = 0)."""
 
-    def __init__(self, in_features, hidden_features=None, out_features=None, shift_size=5):
+    def __init__(self, in_features, hidden_features=None, out_features=None, shift_size=5,
+                 linear="fp32"):
         super().__init__()
+        if linear not in ("fp32", "fp8"):
+            raise ValueError(f"linear must be 'fp32' or 'fp8', got {linear!r}")
+        self.linear = linear
         out_features = out_features or in_features
         hidden_features = hidden_features or in_features
         self.dim = in_features
@@ -206,24 +215,41 @@ class shiftmlp(nn.Module):  # noqa: N801 (reference name)
     def run(self, x):
         """x: [B, H, W, C] tokens -> fc2(shiftW(gelu(dw(fc1(shiftH(x))))))."""
         s = token_shift(x, 0)
-        f1 = ops.pw_conv([s], self.fc1.weight, self.fc1.bias).z
+        f1 = self._linear(s, self.fc1)
         d = ops.dw_conv(f1, self.dwconv.dwconv.weight, self.dwconv.dwconv.bias).z
         s2 = token_shift(gelu(d), 1)
-        return ops.pw_conv([s2], self.fc2.weight, self.fc2.bias).z
+        return self._linear(s2, self.fc2)
+
+    def _linear(self, x, fc):
+        if self.linear == "fp8":
+            return fp8.linear(x, fc.weight, fc.bias)
+        return ops.pw_conv([x], fc.weight, fc.bias).z
 
 
 class shiftedBlock(nn.Module):  # noqa: N801
-    """UNext.py:166-201: x + mlp(norm2(x)) (drop_path 0 -> identity)."""
+    """UNext.py:166-201: x + mlp(norm2(x)) (drop_path 0 -> identity), and the norm that the
+    network has behind the block. sandwich: x + scale * post_norm(mlp(norm2(x))) instead."""
 
-    def __init__(self, dim, mlp_ratio=1.0):
+    def __init__(self, dim, mlp_ratio=1.0, sandwich=False, linear="fp32"):
         super().__init__()
         self.drop_path = nn.Identity()
         self.norm2 = nn.LayerNorm(dim)
-        self.mlp = shiftmlp(in_features=dim, hidden_features=int(dim * mlp_ratio))
+        self.mlp = shiftmlp(in_features=dim, hidden_features=int(dim * mlp_ratio), linear=linear)
+        self.post_norm = nn.LayerNorm(dim) if sandwich else None
+        if sandwich:
+            self.scale = nn.Parameter(torch.ones(dim))
 
-    def run(self, x):
+    def run(self, x, after: nn.LayerNorm = None):
+        """block(x), or after(block(x)) with the norm that follows it"""
         m = self.mlp.run(layernorm(x, self.norm2))
-        return ops.bn_act_add(m, res=x, act_after=ACT_NONE).z
+        post = self.post_norm
+        if post is None:
+            out = ops.bn_act_add(m, res=x, act_after=ACT_NONE).z
+            return out if after is None else layernorm(out, after)
+        if after is None:
+            return sandwich_norm(x, m, post.weight, post.bias, self.scale, pre=False)[0]
+        return sandwich_norm(x, m, post.weight, post.bias, self.scale, None, after.weight,
+                             after.bias, eps=after.eps)[1]
 
 
 class OverlapPatchEmbed(nn.Module):
@@ -246,8 +272,10 @@ class UNext(nn.Module):
     """UNext.py:231-358 (embed_dims 128/160/256, depths 1/1/1, mlp_ratio 1)."""
 
     def __init__(self, n_channels=3, n_classes=1, deep_supervision=False, img_size=224,
-                 patch_size=16, in_chans=3, embed_dims=(128, 160, 256), **kwargs):
+                 patch_size=16, in_chans=3, embed_dims=(128, 160, 256), sandwich=False,
+                 linear="fp32", **kwargs):
         super().__init__()
+        opts = {"sandwich": sandwich, "linear": linear}
         d0, d1, d2 = embed_dims
         self.n_channels, self.n_classes = n_channels, n_classes
         self.encoder1 = nn.Conv2d(n_channels, 16, 3, stride=1, padding=1)
@@ -260,10 +288,10 @@ class UNext(nn.Module):
         self.norm4 = nn.LayerNorm(d2)
         self.dnorm3 = nn.LayerNorm(d1)
         self.dnorm4 = nn.LayerNorm(d0)
-        self.block1 = nn.ModuleList([shiftedBlock(d1)])
-        self.block2 = nn.ModuleList([shiftedBlock(d2)])
-        self.dblock1 = nn.ModuleList([shiftedBlock(d1)])
-        self.dblock2 = nn.ModuleList([shiftedBlock(d0)])
+        self.block1 = nn.ModuleList([shiftedBlock(d1, **opts)])
+        self.block2 = nn.ModuleList([shiftedBlock(d2, **opts)])
+        self.dblock1 = nn.ModuleList([shiftedBlock(d1, **opts)])
+        self.dblock2 = nn.ModuleList([shiftedBlock(d0, **opts)])
         self.patch_embed3 = OverlapPatchEmbed(img_size // 4, 3, 2, d0, d1)
         self.patch_embed4 = OverlapPatchEmbed(img_size // 8, 3, 2, d1, d2)
         self.decoder1 = nn.Conv2d(d2, d1, 3, stride=1, padding=1)
@@ -290,15 +318,13 @@ class UNext(nn.Module):
         t2 = relu(ops.pool2(conv_bn(t1, self.encoder2, self.ebn2)))
         t3 = relu(ops.pool2(conv_bn(t2, self.encoder3, self.ebn3)))
         # tokenized MLP stages (:268-290)
-        out = self.block1[0].run(self.patch_embed3.run(t3))
-        t4 = layernorm(out, self.norm3)
-        out = self.block2[0].run(self.patch_embed4.run(t4))
-        out = layernorm(out, self.norm4)
+        t4 = self.block1[0].run(self.patch_embed3.run(t3), self.norm3)
+        out = self.block2[0].run(self.patch_embed4.run(t4), self.norm4)
         # decoder (:293-351): relu(interp(bn(conv))) + skip
         out = up2_relu_add(conv_bn(out, self.decoder1, self.dbn1), t4)
-        out = layernorm(self.dblock1[0].run(out), self.dnorm3)
+        out = self.dblock1[0].run(out, self.dnorm3)
         out = up2_relu_add(conv_bn(out, self.decoder2, self.dbn2), t3)
-        out = layernorm(self.dblock2[0].run(out), self.dnorm4)
+        out = self.dblock2[0].run(out, self.dnorm4)
         out = up2_relu_add(conv_bn(out, self.decoder3, self.dbn3), t2)
         out = up2_relu_add(conv_bn(out, self.decoder4, self.dbn4), t1)
         out = up2_relu_add(ops.conv3x3(out, self.decoder5.weight, self.decoder5.bias).z)
