@@ -95,6 +95,23 @@ int main() {
   float* one = reinterpret_cast<float*>(16);
   EXPECT(accunet_dw3x3_fwd(one, one, nullptr, nullptr, nullptr, 0, 1, one, nullptr, 1, 8, 8, 32,
                            one, nullptr, 0, 0, nullptr) == -2);
+  // token-block operators: workspace sizes over lengths from one to long, refusals
+  const long lens[] = {1, 2, 127, 128, 129, 1001, 16384, 70001};
+  for (long m : lens)
+    for (long k : lens)
+      for (int flags = 0; flags < 4; ++flags) {
+        EXPECT(accunet_fp8_linear_ws_bytes(m, 333, k, flags & 1) > 0);
+        EXPECT((accunet_fp8_linear_save_bytes(m, 333, k, flags & 1, flags >> 1) > 0) == (flags != 0));
+        EXPECT(accunet_fp8_linear_bwd_ws_bytes(m, 333, k, 1, flags & 1, flags >> 1) > 0);
+        EXPECT(accunet_distill_save_bytes(m, 1, (int)k, 1 + flags) > 0);
+        EXPECT(accunet_distill_ws_bytes(m, 1, (int)k, 1 + flags, flags & 1) > 0);
+        if (k <= 8192) EXPECT(accunet_blocknorm_ws_elems(m * 3, m, (int)k, flags % 3) > 0);
+        sink += accunet_distill_fused(m, 1, (int)k, flags & 1);
+      }
+  EXPECT(accunet_blocknorm_ws_elems(5, 2, 8, 0) == 0);
+  EXPECT(accunet_distill_save_bytes(2, 1, 5, 257) == 0);
+  EXPECT(accunet_fp8_linear_ws_bytes(0, 8, 8, 1) == 0);
+  EXPECT(accunet_fp8_quantize(one, 0, one, nullptr, nullptr, nullptr, 2, 8, 0, nullptr) == -2);
   EXPECT(accunet_abi_hash() != 0);
   std::printf("asan_abi: %d failure(s), checksum %ld\n", fails, sink);
   return fails ? 1 : 0;
