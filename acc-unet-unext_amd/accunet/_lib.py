@@ -156,6 +156,7 @@ _SIGS = {
     "accunet_blocknorm_fwd": [P, P, P, P, P, P, I, P, P, I, F, P, P, P, L, L, I, I, P],
     "accunet_blocknorm_ws_elems": [L, L, I, I],
     "accunet_blocknorm_bwd": [P, P, P, P, P, P, I, P, I, P, P, P, P, P, P, P, P, S, L, L, I, I, P],
+    "accunet_stream_capture_id": [P],
     "accunet_distill_save_bytes": [L, L, I, I],
     "accunet_distill_ws_bytes": [L, L, I, I, I],
     "accunet_distill_fused": [L, L, I, I],
@@ -176,7 +177,7 @@ _SIZE_FNS = {"accunet_bn_bwd_ws_elems", "accunet_bn_bwd_part_ws_elems", "accunet
              "accunet_fp8_linear_save_bytes", "accunet_fp8_linear_ws_bytes",
              "accunet_fp8_linear_bwd_ws_bytes"}
 
-_LL_FNS = {"accunet_abi_hash", "accunet_conv3x3_halo_launches"}
+_LL_FNS = {"accunet_abi_hash", "accunet_conv3x3_halo_launches", "accunet_stream_capture_id"}
 HEADER = os.path.join(os.path.dirname(os.path.dirname(_HERE)), "include", "accunet.h")
 
 _lib = None

@@ -39,13 +39,16 @@ def _forward(z, idx, top, rest, T, weight, reduction, B, S, V, K, dz):
 class _DistillFn(torch.autograd.Function):
     """The forward writes the gradient for an upstream of 1 where one kernel can do both
     (sum and mean), and the backward hands that tensor out, once: its kernel rewrites it only
-    for another upstream gradient. A further backward of the same graph computes it anew."""
+    for another upstream gradient. A further backward of the same graph computes it anew, and
+    so does a backward in another graph capture than the forward's: replayed by itself, it
+    would hand out what the consumers of the last replay left in that tensor."""
 
     @staticmethod
     def forward(ctx, z, idx, top, rest, T, weight, reduction, B, S, V, K):
         fuse = reduction != 0 and B * S > 0 and kern.distill_fused(B, S, V, kern._dt(z))
         ctx.dz = torch.empty_like(z) if fuse else None
         loss, save = _forward(z, idx, top, rest, T, weight, reduction, B, S, V, K, ctx.dz)
+        ctx.capture = kern.capture_id(z)
         ctx.save_for_backward(z, save)
         ctx.cfg = (reduction, B, S, V, K, T, weight)
         return loss
@@ -55,7 +58,7 @@ class _DistillFn(torch.autograd.Function):
     def backward(ctx, up):
         z, save = ctx.saved_tensors
         dz, ctx.dz = ctx.dz, None
-        held = dz is not None
+        held = dz is not None and ctx.capture == kern.capture_id(z) >= 0
         if not held:
             dz = torch.empty_like(z)
         if save is not None:

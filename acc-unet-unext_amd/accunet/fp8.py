@@ -43,6 +43,14 @@ class Fp8Blocks:
     __slots__ = ("q", "s", "rows", "cols", "square", "t")
 
     def __init__(self, q, s, rows, cols, square, t=None):
+        for name, a, dtype, shape in (("q", q, torch.float8_e4m3fn, (rows, _pad(cols))),
+                                      ("s", s, torch.uint8, (rows, _pitch(cols)))):
+            if a.dtype != dtype or tuple(a.shape) != shape or not a.is_contiguous():
+                raise AccError(f"Fp8Blocks: {name} {a.dtype} {tuple(a.shape)}, expected a "
+                               f"contiguous {dtype} {shape}")
+        if q.device != s.device or (t is not None and (t.shape != (cols, rows) or
+                                                       t.device != q.device)):
+            raise AccError("Fp8Blocks: q, s and the transposed matrix do not belong together")
         self.q, self.s, self.rows, self.cols, self.square, self.t = q, s, rows, cols, square, t
 
     @property

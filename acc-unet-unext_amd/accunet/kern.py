@@ -645,6 +645,11 @@ def distill_fused(B, S, V, dt) -> bool:
     return bool(_lib.load().accunet_distill_fused(B, S, V, dt))
 
 
+def capture_id(t) -> int:
+    """The graph capture that the current stream of t's device is part of; 0: none."""
+    return _lib.load().accunet_stream_capture_id(torch._C._cuda_getCurrentRawStream(t.get_device()))
+
+
 def distill_fwd(z, idx, top, rest, loss, reduction, dz, B, S, V, K, T, weight):
     """The loss (and dz for an upstream of 1, where given); returns what a backward needs."""
     lib, dt = _lib.load(), _dt(z)

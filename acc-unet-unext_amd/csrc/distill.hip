@@ -402,6 +402,17 @@ extern "C" size_t accunet_distill_ws_bytes(long B, long S, int V, int K, int dt)
   DtArgs a = dt_args(B, S, V, K, 1.f, 1.f);
   return (size_t)dt_carve_ws(a, nullptr, dt);
 }
+// the capture that `stream` is part of, 0 outside one (the null stream is never captured)
+extern "C" long long accunet_stream_capture_id(void* stream) {
+  if (!stream) return 0;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return -1;
+  }
+  return status == hipStreamCaptureStatusActive ? (long long)id : 0;
+}
 // one block a row (or pixel), so the gradient can follow the sum in the same kernel
 extern "C" int accunet_distill_fused(long B, long S, int V, int dt) {
   return dt_planes(S) || dt_rows_runs(B, V, dt) == 1;

@@ -531,6 +531,9 @@ int accunet_blocknorm_bwd(const void* x, const void* f, const float* w1, const f
  *     gradient `up` (one value, one a row with reduction 0). held != 0: dz is the tensor that
  *     the forward filled; it is rewritten only where `up` is not what it holds.
  * ------------------------------------------------------------------------- */
+/* identity of the graph capture that `stream` is part of, 0 outside one (a forward's dz may be
+ * handed to accunet_distill_bwd as held only within the same capture, or outside any) */
+long long accunet_stream_capture_id(void* stream);
 size_t accunet_distill_save_bytes(long B, long S, int V, int K);
 size_t accunet_distill_ws_bytes(long B, long S, int V, int K, int dt);
 int accunet_distill_fused(long B, long S, int V, int dt);

@@ -395,12 +395,14 @@ def test_backward_alone_captured():
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             (dz,) = torch.autograd.grad(loss, zz, up)
+            out = dz.clone()
+            dz.add_(1.0)  # a consumer that works in place
     for u in (2.0, 1.0, 1.0, 0.5, 1.0):
         up.fill_(u)
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(dz, want[u]), u
+        assert torch.equal(out, want[u]), u
 
 
 @pytest.mark.gpu

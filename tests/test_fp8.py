@@ -29,6 +29,12 @@ def test_refusals_on_the_host():
         fp8.quantize(torch.zeros(2, 8))
     with pytest.raises(_lib.AccError):
         fp8.linear(torch.zeros(2, 8), torch.zeros(4, 8))
+    q, s = torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.full((4, 4), 127, dtype=torch.uint8)
+    assert fp8.Fp8Blocks(q, s, 4, 77, True).shape == (4, 77)
+    for bad in ((q[:3], s, 4, 77), (q, s[:, :3], 4, 77), (q, s, 4, 129), (q.float(), s, 4, 77),
+                (q.t(), s, 128, 4), (s, q, 4, 77)):
+        with pytest.raises(_lib.AccError):
+            fp8.Fp8Blocks(*bad, True)
     lib = _lib.load()
     ok = 16
     q = lib.accunet_fp8_quantize

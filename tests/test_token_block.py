@@ -153,3 +153,26 @@ def test_unext_options_train():
     grads = dict(zip(names, out[0][1:]))
     for n in ("block1.0.mlp.fc1.weight", "block2.0.scale", "dblock1.0.post_norm.weight"):
         assert float(grads[n].abs().max()) > 0, n
+
+
+@pytest.mark.gpu
+def test_unext_options_in_a_captured_step():
+    """TrainStep's graph mode with the options on: three replayed steps give the eager
+    steps' losses and parameters bit for bit."""
+    from accunet.train import TrainStep
+    from accunet.unext import UNext
+    gen = torch.Generator().manual_seed(3)
+    xs = [torch.randn(2, 3, 64, 64, generator=gen).cuda() for _ in range(3)]
+    ys = [(torch.rand(2, 1, 64, 64, generator=gen) < 0.4).float().cuda() for _ in range(3)]
+    torch.manual_seed(0)
+    state = UNext(3, 1, sandwich=True, linear="fp8").state_dict()
+    runs = []
+    for graph in (True, False):
+        m = UNext(3, 1, sandwich=True, linear="fp8")
+        m.load_state_dict(state)
+        step = TrainStep(m.cuda().train(), lr=1e-3, graph=graph)
+        losses = [float(step(x, y)) for x, y in zip(xs, ys)]
+        runs.append((losses, [p.detach().clone() for p in m.parameters()]))
+        del step, m
+    assert runs[0][0] == runs[1][0]
+    assert all(torch.equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
