@@ -60,6 +60,28 @@ ACC_DEV void dt_load(const T* z, int off, int V, int q, float (&v)[DtVec<T>::N])
     for (int u = 0; u < N; ++u) v[u] = j + u >= 0 && j + u < V ? ld1(z + j + u) : -INFINITY;
   }
 }
+// A row's whole vectors: [lo, hi) of its nq, and its aligned base. What a wave reads between
+// them needs no look at the row's ends.
+template <typename T>
+struct DtRun {
+  const acc_u32x4* base;
+  int lo, hi;
+  ACC_DEV DtRun(const T* z, int off, int V) {
+    constexpr int N = DtVec<T>::N;
+    base = reinterpret_cast<const acc_u32x4*>(z - off);
+    lo = off ? 1 : 0;
+    hi = (off + V) / N;
+  }
+  // vectors q, q + step, .. (n of them) of every lane of the wave, q0 the first lane's q
+  ACC_DEV bool whole(int q0, int step, int n, int end) const {
+    return q0 >= lo && q0 + (n - 1) * step + 64 <= min(hi, end);
+  }
+};
+template <typename T>
+ACC_DEV float dt_get(const acc_u32x4& w, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+  else return e & 1 ? bfhi(w[e >> 1]) : bflo(w[e >> 1]);
+}
 template <typename T>
 ACC_DEV int dt_offset(const T* p) { return (int)(((uintptr_t)p & 15) / sizeof(T)); }
 
@@ -106,32 +128,17 @@ ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id
                        unsigned* mark, float c, float& m, float& s) {
   constexpr int N = DtVec<T>::N;
   constexpr int U = sizeof(T) == 4 ? 4 : 2;  // vectors in flight a thread
+  const DtRun<T> run(z, off, V);
   for (int qc = q0; qc < q1; qc += DTR_CHUNK) {
     const int qe = min(q1, qc + DTR_CHUNK);
     if (REST) dt_marks<N, NT>(mark, qc, qe, id, K, off, t);
-    for (int q = qc + t; q < qe; q += NT * U) {
-      float v[U][N];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (q + u * NT < qe) dt_load(z, off, V, q + u * NT, v[u]);
-        else
-#pragma unroll
-          for (int e = 0; e < N; ++e) v[u][e] = -INFINITY;
-      if (REST) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (q + u * NT >= qe) continue;
-          const unsigned bits = dt_mark(mark, q + u * NT - qc);
-          if (bits)
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[u][e] = (bits >> e) & 1u ? -INFINITY : v[u][e];
-        }
-      }
-      float mv = v[0][0];
+    // sums U vectors, get(u, e) a class
+    auto add = [&](auto get) {
+      float mv = get(0, 0);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < N; ++e) mv = fmaxf(mv, v[u][e]);
+        for (int e = 0; e < N; ++e) mv = fmaxf(mv, get(u, e));
       if (mv > m) {
         s *= dt_rescale(m, mv, c);
         m = mv;
@@ -140,7 +147,39 @@ ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += dt_exp2(__builtin_fmaf(v[u][e], c, -ref));
+        for (int e = 0; e < N; ++e) s += dt_exp2(__builtin_fmaf(get(u, e), c, -ref));
+    };
+    for (int q = qc + t; q < qe; q += NT * U) {
+      if (run.whole(__builtin_amdgcn_readfirstlane(q), NT, U, qe)) {
+        acc_u32x4 w[U];
+        unsigned bits[U], any = 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = run.base[q + u * NT];
+        if (REST)
+#pragma unroll
+          for (int u = 0; u < U; ++u) any |= bits[u] = dt_mark(mark, q + u * NT - qc);
+        if (!REST || !__any(any)) {
+          add([&](int u, int e) { return dt_get<T>(w[u], e); });
+        } else {
+          add([&](int u, int e) { return (bits[u] >> e) & 1u ? -INFINITY : dt_get<T>(w[u], e); });
+        }
+        continue;
+      }
+      float v[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (q + u * NT < qe) {
+          dt_load(z, off, V, q + u * NT, v[u]);
+          const unsigned bits = REST ? dt_mark(mark, q + u * NT - qc) : 0u;
+          if (REST && bits)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[u][e] = (bits >> e) & 1u ? -INFINITY : v[u][e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[u][e] = -INFINITY;
+        }
+      }
+      add([&](int u, int e) { return v[u][e]; });
     }
   }
 }
@@ -330,10 +369,12 @@ distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
 // are fetched at the start, beside the stream, and marked in LDS for the whole row where it
 // has at most DTR_CHUNK vectors: the gradient then goes around them and they are written
 // without waiting for it.
-// The gradient's second read of the row finds little of it in the caches: the rows in
-// flight are larger than the L2 (4096 x 128000 bf16: 522 us, three passes at 6 TB/s). Held
-// in registers instead (64 a thread for the row, one block a CU) it took 592-860 us: sums,
-// barriers and stores of one row then stand one behind another on each CU.
+// The gradient's second read of the row misses the L2 but not the last-level cache (4096 x
+// 128000 bf16: 1.05 GB fetched from memory, 1.06 GB written), so two reads and a write cross
+// the fabric: 3.15 GB in 486-518 us, 6.1-6.5 TB/s, what a copy reaches. Loads a step ahead
+// (488-571 us) or the row from its end changed nothing. Held in registers instead (64 a
+// thread for the row, one block a CU) it took 592-860 us: sums, barriers and stores of one
+// row then stand one behind another on each CU.
 template <typename T, bool REST, int NT, bool STREAM>
 __global__ void __launch_bounds__(NT)
 distill_rows_fused_kernel(const DtArgs a, const DtScale g) {
@@ -400,17 +441,36 @@ distill_rows_fused_kernel(const DtArgs a, const DtScale g) {
   }
   if (my >= 0) dt_put_listed(zr, dr, my, mp, st, a.c, gs);
   constexpr int U = sizeof(T) == 4 ? 4 : 2;
+  const DtRun<T> run(zr, off, V);
   for (int q = t; q < nq; q += NT * U) {
-    float v[U][N];
+    if (run.whole(__builtin_amdgcn_readfirstlane(q), NT, U, nq)) {
+      acc_u32x4 w[U];
+      unsigned bits[U], any = 0u;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (q + u * NT < nq) dt_load(zr, off, V, q + u * NT, v[u]);
+      for (int u = 0; u < U; ++u) {
+        w[u] = run.base[q + u * NT];
+        any |= bits[u] = dt_mark(mark, q + u * NT);
+      }
+      const bool plain = !__any(any);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          v[e] = dt_exp2(__builtin_fmaf(dt_get<T>(w[u], e), a.c, -st.x)) * cu;
+        if (plain) DtVec<T>::template st<STREAM>(dr + (q + u * NT) * N - off, v);
+        else dt_put<T, STREAM>(dr, off, V, q + u * NT, bits[u], v);
+      }
+      continue;
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (q + u * NT >= nq) continue;
+      float v[N];
+      dt_load(zr, off, V, q + u * NT, v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[u][e] = dt_exp2(__builtin_fmaf(v[u][e], a.c, -st.x)) * cu;
-      dt_put<T, STREAM>(dr, off, V, q + u * NT, dt_mark(mark, q + u * NT), v[u]);
+      for (int e = 0; e < N; ++e) v[e] = dt_exp2(__builtin_fmaf(v[e], a.c, -st.x)) * cu;
+      dt_put<T, STREAM>(dr, off, V, q + u * NT, dt_mark(mark, q + u * NT), v);
     }
   }
 }
