@@ -258,6 +258,14 @@ def test_strides_empty_rows_and_refusals():
     kappa = y64.abs().amax(-1, keepdim=True) * rstd + want.abs().amax(-1, keepdim=True)
     for t in (y, y.clone()):
         _compare("h", bn.norm(t), want, 128 * U * (want.abs() + kappa))
+    # one row without a batch axis; another stream
+    assert torch.equal(bn.norm(f[0, 0]), bn.norm(f)[0, 0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        r3, h3 = bn.sandwich_norm(x, f)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(r, r3) and torch.equal(h, h3)
     # constant rows: zero variance
     c = torch.full((2, 48), 3.0, device="cuda", requires_grad=True)
     hc = bn.norm(c)

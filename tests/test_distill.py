@@ -269,6 +269,13 @@ def test_types_strides_and_module():
     img = z.float().view(3, 4, 700).movedim(-1, 1).reshape(3, 700, 2, 2)
     ii, tt = (t.view(3, 4, 9).movedim(-1, 1).reshape(3, 9, 2, 2) for t in (idx, top))
     c = m(img, ii, tt, r.view(3, 2, 2))
+    assert torch.equal(c, m(img, ii.int(), tt.float(), r.view(3, 2, 2)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c2 = m(img, ii, tt, r.view(3, 2, 2))
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(c, c2)
     d = f(z.float(), idx, top, rest=r, temperature=2.0)
     assert abs(float(c) - float(d)) <= 1e-5 * abs(float(d))
     with pytest.raises(_lib.AccError):

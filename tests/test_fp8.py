@@ -288,6 +288,19 @@ def test_shapes_strides_partial_gradients_and_refusals():
         got = torch.autograd.grad(fp8.linear(*args), on, dy)
         for g, wnt in zip(got, [w for i, w in enumerate(want) if mask >> i & 1]):
             assert torch.equal(g, wnt)
+    # the bias alone over a frozen weight, one token without a batch axis, another stream
+    bias = m.bias.detach().clone().requires_grad_()
+    frozen = fp8.quantize(m.weight, square=True)
+    y = fp8.linear(x, frozen, bias)
+    assert torch.equal(torch.autograd.grad(y, bias, dy)[0], want[2])
+    one = fp8.linear(x[0, 0], frozen, bias)
+    assert one.shape == (24,) and torch.equal(one, fp8.linear(x[0, :1], frozen, bias)[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z = fp8.linear(x, frozen, bias)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(z, y)
     # no tokens
     e = torch.empty(0, 64, device="cuda", requires_grad=True)
     m.zero_grad()
