@@ -63,7 +63,8 @@ class Fp8Blocks:
 
     def values(self):
         """The float32 values that the matrix stands for."""
-        scale = torch.ldexp(torch.ones((), device=self.device), self.s.int() - 127)
+        # from its bits: torch.ldexp's powers of two are not exact on the GPU
+        scale = (self.s.int() << 23).view(torch.float32)
         scale = scale.repeat_interleave(BLOCK, 1)[:, :self.cols]
         return self.q[:, :self.cols].float() * scale
 

@@ -140,6 +140,15 @@ def test_quantize(R, C, dtype):
 
 
 @pytest.mark.gpu
+def test_values_of_every_scale():
+    fp8 = _mod()
+    x = torch.ldexp(torch.ones(246, 1), torch.arange(246).view(-1, 1) - 126 + 8) * 1.75
+    b = fp8.quantize(x.cuda())
+    assert torch.equal(b.s[:, 0].int().cpu(), torch.arange(1, 247, dtype=torch.int32))
+    assert torch.equal(b.values().cpu(), x) and bool((b.q[:, 0].float() == 448).all())
+
+
+@pytest.mark.gpu
 def test_quantize_values_at_the_edges():
     """Ties, the largest value and its neighbours, subnormals of e4m3 and of fp32, zeros,
     infinities and NaN, the largest and smallest fp32 scales."""
