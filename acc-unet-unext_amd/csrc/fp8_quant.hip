@@ -194,9 +194,14 @@ void fp8_quantize(const void* x, int dt, bool square, unsigned char* q, unsigned
   with_dt(dt, [&](auto tag) {
     using T = decltype(tag);
     if (!square && !qt && !sum) {
-      const long n = R * SP * 16;
-      hipLaunchKernelGGL(fp8_rows_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, str,
-                         (const T*)x, q, s, R, C, CP, SP);
+      // a launch holds fewer than 2^32 threads
+      const long most = (1L << 31) / (SP * 16);
+      for (long r = 0; r < R; r += most) {
+        const long rows = min(most, R - r);
+        hipLaunchKernelGGL(fp8_rows_kernel<T>, dim3((unsigned)((rows * SP * 16 + 255) / 256)),
+                           dim3(256), 0, str, (const T*)x + r * C, q + r * CP, s + r * SP, rows, C,
+                           CP, SP);
+      }
       return;
     }
     hipLaunchKernelGGL(fp8_tile_kernel<T>, dim3((unsigned)(RP / 128), CP / 128), dim3(256), 0, str,

@@ -149,6 +149,23 @@ def test_values_of_every_scale():
 
 
 @pytest.mark.gpu
+def test_quantize_more_rows_than_a_launch_holds():
+    """2^26 rows of one block take 2^32 threads: the rows on both sides of a cut, and the
+    first and last, are what a call on these rows alone gives."""
+    fp8 = _mod()
+    R, C = 2 ** 26 + 3, 3
+    x = torch.empty(R, C, dtype=torch.bfloat16, device="cuda")
+    x.view(torch.int16).copy_(torch.arange(R * C, device="cuda").view(R, C) * 77 % 16256)
+    b = fp8.quantize(x)
+    for r in (0, 2 ** 25 - 40, 2 ** 26 - 77):
+        part = fp8.quantize(x[r:r + 80])
+        n = part.rows
+        assert torch.equal(b.q[r:r + n].view(torch.uint8), part.q.view(torch.uint8))
+        assert torch.equal(b.s[r:r + n], part.s)
+        _assert_blocks(part, x[r:r + n], 1)
+
+
+@pytest.mark.gpu
 def test_quantize_values_at_the_edges():
     """Ties, the largest value and its neighbours, subnormals of e4m3 and of fp32, zeros,
     infinities and NaN, the largest and smallest fp32 scales."""
