@@ -77,7 +77,8 @@ def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight
     reduction: "mean" over the rows that have an entry, "sum", or "none" (one loss a row).
     `weight` multiplies the loss (inside: a factor applied to the result, 0.5 * loss, costs the
     backward another pass over the logits). Non-contiguous inputs are copied, and so are more than
-    1024 classes on dim=1."""
+    1024 classes on dim=1. At most 2^26 - 4 rows with the classes last, 2^24 - 1 above 2032
+    classes."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     temperature, weight = float(temperature), float(weight)

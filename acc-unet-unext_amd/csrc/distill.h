@@ -129,6 +129,10 @@ struct DtArgs {
 // rows with the classes last (distill_rows.hip); up to DTR_WAVE_V classes a wave has a row
 // in registers (512 vectors of 4 fp32 at most, partial ones at both ends included)
 #define DTR_WAVE_V 2032
+// a launch holds fewer than 2^32 threads: 64 a row, 256 a long one (the 512 and 1024 of rows
+// above 64 KB and 128 KB end at 550 GB of logits)
+#define DTR_WAVE_ROWS ((1L << 26) - 4)
+#define DTR_LONG_ROWS ((1L << 24) - 1)
 int dt_rows_runs(long R, int V, int dt);
 void dt_rows_forward(const DtArgs& a, int dt, hipStream_t st);
 void dt_rows_backward(const DtArgs& a, const DtScale& g, int dt, hipStream_t st);

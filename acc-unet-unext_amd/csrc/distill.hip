@@ -382,6 +382,7 @@ static int dt_check(long B, long S, int V, int K, float T) {
   if (B <= 0 || S <= 0 || B * S > 0x7fffffffL || V <= 0 || V > DT_MAX_V || K <= 0 || K > DT_MAX_K)
     return ACC_EBADSHAPE;
   if (dt_planes(S) && V > DTP_MAX_V) return ACC_EBADSHAPE;
+  if (!dt_planes(S) && B > (V <= DTR_WAVE_V ? DTR_WAVE_ROWS : DTR_LONG_ROWS)) return ACC_EBADSHAPE;
   return T > 0.f && T < INFINITY ? ACC_OK : ACC_EBADARG;
 }
 static DtArgs dt_args(long B, long S, int V, int K, float T, float weight) {

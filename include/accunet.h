@@ -525,8 +525,9 @@ int accunet_blocknorm_bwd(const void* x, const void* f, const float* w1, const f
  *   accunet_distill_fwd: loss (one value; one a row with reduction 0). reduction: 0 none, 1
  *     sum, 2 mean over the rows with an entry. S = 1 for "rows" (B = R). save (kept for the
  *     backward) and ws (scratch): accunet_distill_save_bytes / _ws_bytes bytes; z, save and
- *     ws are 16-byte aligned. dz (or NULL; reduction 1, 2 and accunet_distill_fused only): the gradient for
- *     an upstream gradient of 1 in the same pass.
+ *     ws are 16-byte aligned. dz (or NULL; reduction 1, 2 and accunet_distill_fused only): the
+ *     gradient for an upstream gradient of 1 in the same pass. At most 2^31 - 1 pixels (B * S)
+ *     in planes, 2^26 - 4 rows, or 2^24 - 1 above 2032 classes.
  *   accunet_distill_bwd: dz (z's type, shape and address modulo 16) scaled by the upstream
  *     gradient `up` (one value, one a row with reduction 0). held != 0: dz is the tensor that
  *     the forward filled; it is rewritten only where `up` is not what it holds.

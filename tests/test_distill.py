@@ -57,6 +57,22 @@ def test_refusals_on_the_host():
     assert lib.accunet_distill_fused(3, 1, 2048, 0) == 1 and lib.accunet_distill_fused(2, 9, 5, 0) == 1
 
 
+def test_more_rows_than_a_launch_holds_are_refused():
+    """A launch holds fewer than 2^32 threads: 64 for a row, 256 for one of more than 2032
+    classes; pixels of a plane take one each."""
+    lib = _lib.load()
+    for V, most in ((9, 2 ** 26 - 4), (2032, 2 ** 26 - 4), (2033, 2 ** 24 - 1)):
+        assert lib.accunet_distill_save_bytes(most, 1, V, 1) > 0
+        assert lib.accunet_distill_save_bytes(most + 1, 1, V, 1) == 0
+        assert lib.accunet_distill_ws_bytes(most + 1, 1, V, 1, 0) == 0
+        assert lib.accunet_distill_fwd(16, 16, 1, 16, 0, None, 16, 2, None, 16, 2 ** 62, 16, 2 ** 62,
+                                       most + 1, 1, V, 1, 1.0, 1.0, 0, None) == -1
+        assert lib.accunet_distill_bwd(16, 16, 2 ** 62, 16, 2, 0, 16, most + 1, 1, V, 1, 1.0, 1.0,
+                                       0, None) == -1
+    assert lib.accunet_distill_save_bytes(1, 2 ** 31 - 1, 9, 1) > 0
+    assert lib.accunet_distill_save_bytes(1, 2 ** 31, 9, 1) == 0
+
+
 # ----------------------------------------------------------------------- the reference
 def _reference(z, idx, top, rest, T, weight=1.0):
     """Per-row loss and gradient (unit upstream) in 64 bits, rows [R][V], with bounds."""
