@@ -176,3 +176,68 @@ def test_unext_options_in_a_captured_step():
         del step, m
     assert runs[0][0] == runs[1][0]
     assert all(torch.equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
+
+
+def _near(big, small):
+    """Two calls on the same rows: one bf16 step apart at most, 2^-13 of the largest value on
+    top for fp32 sums in another order (up to 2^11 terms, 2^-24 each)."""
+    a, b = big.detach().double(), small.detach().double()
+    bound = torch.finfo(torch.bfloat16).eps * b.abs() + 2.0 ** -13 * float(b.abs().max())
+    assert float(b.abs().max()) > 0 and bool(((a - b).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["norm", "rows", "planes", "linear"])
+def test_offsets_past_32_bits(op):
+    """More than 2^31 elements: the last rows are what a call on these rows alone gives."""
+    from accunet import blocknorm, distill, fp8
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def rand(*shape):
+        return torch.empty(*shape, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+
+    n = 300
+
+    def leaf(t):
+        return t.detach().clone().requires_grad_()
+
+    if op == "norm":
+        P, C = 2 ** 22 + 3, 520
+        x, f = rand(P, C).requires_grad_(), rand(P, C).requires_grad_()
+        r, h = blocknorm.sandwich_norm(x, f)
+        torch.autograd.backward([r, h], [x.detach(), f.detach()])
+        xs, fs = leaf(x[-n:]), leaf(f[-n:])
+        rs, hs = blocknorm.sandwich_norm(xs, fs)
+        torch.autograd.backward([rs, hs], [xs.detach(), fs.detach()])
+        for a, b in ((r, rs), (h, hs), (x.grad, xs.grad), (f.grad, fs.grad)):
+            _near(a[-n:], b)
+    elif op == "linear":
+        M, K, N = 2 ** 21 + 300, 1040, 8
+        x = rand(M, K).requires_grad_()
+        w = torch.randn(N, K, generator=g, device="cuda", requires_grad=True)
+        first = (M - n) // 128 * 128  # the first of a block of 128 tokens
+        dy = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+        dy[first:].normal_(generator=g)
+        y = fp8.linear(x, w)
+        y.backward(dy)
+        xs, ws = leaf(x[first:]), leaf(w)
+        ys = fp8.linear(xs, ws)
+        ys.backward(dy[first:])
+        for a, b in ((y[first:], ys), (x.grad[first:], xs.grad), (w.grad, ws.grad)):
+            _near(a, b)
+        assert not x.grad[:first].any()
+    else:
+        shape, dim = ((2 ** 21 + 70001, 1001), -1) if op == "rows" else ((4, 21, 2 ** 25 + 5), 1)
+        K = [s if i != dim % len(shape) else 2 for i, s in enumerate(shape)]
+        z = rand(*shape).requires_grad_()
+        V = shape[dim]
+        idx = torch.randint(0, V, K, generator=g, device="cuda", dtype=torch.int32)
+        top = rand(*K)
+        loss = distill.topk_distill(z, idx, top, reduction="none", dim=dim)
+        loss.backward(torch.ones_like(loss))
+        cut = (slice(-n, None),) if op == "rows" else (slice(3, 4), slice(None), slice(-n, None))
+        zs = leaf(z[cut])
+        ls = distill.topk_distill(zs, idx[cut], top[cut], reduction="none", dim=dim)
+        ls.backward(torch.ones_like(ls))
+        _near(loss[-n:] if op == "rows" else loss[3:, -n:], ls)
+        _near(z.grad[cut], zs.grad)
