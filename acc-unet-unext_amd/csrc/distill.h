@@ -10,12 +10,14 @@
 // A row without a valid entry (or whose valid t are all -inf) has loss 0 and gradient 0
 // and is not counted by the mean.
 //
-// Arithmetic is in base 2: with c = log2(e) / T a softmax term is 2^(z*c - m*c), one fma
-// and one v_exp_f32; m*c is rounded once and enters numerator and sum alike, so it cancels.
+// Arithmetic is in base 2: with c = log2(e) / T a softmax term is 2^((z - m)*c), a difference,
+// a product and one v_exp_f32. Of the difference, not z*c - m*c: each thread and block sums
+// relative to its own m, and what rounding m*c loses grows with the logits' offset from zero
+// and differs from one to the next; and the lowest value of a type times c may pass fp32's.
 // q_rest is summed over the classes not listed, never as 1 - sum of the others, and a row's
 // state keeps it relative to the largest such class, so it may be far below fp32's range:
-//   not listed: dz = 2^(z*c - mu) * cu,  cu = 2^(mu - m) / S - rest / S_rest
-//   listed:     dz = 2^(z*c - m) / S - p
+//   not listed: dz = 2^((z - mu)*c) * cu,  cu = 2^((mu - m)*c) / S - rest / S_rest
+//   listed:     dz = 2^((z - m)*c) / S - p
 #pragma once
 #include "common.h"
 
@@ -25,14 +27,16 @@
 #define DT_LOG2E 1.4426950408889634
 
 // one row's state between the passes
-//   x: mu, y: cu, z: m (all * c, base 2), w: 1/S, or DT_EMPTY for a row that does not count
+//   x: mu, y: cu, z: m (logits), w: 1/S, or DT_EMPTY for a row that does not count
 #define DT_EMPTY (-1.f)
 
 ACC_DEV float dt_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 // 2^((m - M) * c), 1 where both are the same infinity
 ACC_DEV float dt_rescale(float m, float M, float c) { return m == M ? 1.f : dt_exp2((m - M) * c); }
-// m * c as a reference for exponents; 0 where no class is left (every term is 2^-inf then)
-ACC_DEV float dt_ref(float m, float c) { return m == -INFINITY ? 0.f : m * c; }
+// m as the reference of terms; 0 where no class is left (every term is 2^-inf then)
+ACC_DEV float dt_ref(float m) { return m == -INFINITY ? 0.f : m; }
+// 2^((z - ref) * c)
+ACC_DEV float dt_term(float z, float ref, float c) { return dt_exp2((z - ref) * c); }
 // (m, s) joined with (m2, s2)
 ACC_DEV void dt_join(float& m, float& s, float m2, float s2, float c) {
   const float M = fmaxf(m, m2);
@@ -75,7 +79,7 @@ struct DtRow {
 };
 ACC_DEV DtRow dt_row_state(float m, float s, float mr, float sr, float rest, bool has_rest, float c) {
   DtRow o;
-  const float ref = dt_ref(m, c);
+  const float ref = dt_ref(m);
   o.M = ref;
   o.log2S = log2f(s);
   o.state.z = ref;
@@ -83,10 +87,17 @@ ACC_DEV DtRow dt_row_state(float m, float s, float mr, float sr, float rest, boo
   o.state.x = ref;
   o.state.y = o.state.w;
   if (has_rest) {
-    o.state.x = dt_ref(mr, c);
+    o.state.x = dt_ref(mr);
     o.state.y = sr > 0.f ? dt_rescale(mr, m, c) / s - rest / sr : (sr == 0.f ? 0.f : sr);
   }
   return o;
+}
+// log2 of q of a class with logit z, and of all classes not listed
+ACC_DEV float dt_log2q(float z, const DtRow& o, float c) {
+  return __builtin_fmaf(z - o.M, c, -o.log2S);
+}
+ACC_DEV float dt_log2q_rest(float mr, float sr, const DtRow& o, float c) {
+  return sr == 0.f ? -INFINITY : __builtin_fmaf(dt_ref(mr) - o.M, c, log2f(sr) - o.log2S);
 }
 
 // the step from a row's sums to its gradient: weight * T * upstream / rows counted

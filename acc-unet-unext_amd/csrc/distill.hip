@@ -45,11 +45,11 @@ distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ t
   }
   mx = dt_wave_max(mx);
   const bool live = __any(any);
-  const float ref = dt_ref(mx, c);
+  const float ref = dt_ref(mx);
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < DT_MAX_K / 64; ++i)
-    if (my[i] >= 0) sum += dt_exp2(__builtin_fmaf(a[i], c, -ref));
+    if (my[i] >= 0) sum += dt_term(a[i], ref, c);
   sum = dt_wave_sum(sum);
   const float r = in && live && rest ? rest[row] : 0.f;
   const float keep = 1.f - r, lg = log2f(sum) - log2f(keep);
@@ -58,7 +58,7 @@ distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ t
   for (int i = 0; i < DT_MAX_K / 64; ++i) {
     const int k = i * 64 + lane;
     if (i >= NI || k >= K) continue;
-    const float e = __builtin_fmaf(a[i], c, -ref);
+    const float e = (a[i] - ref) * c;
     const float v = my[i] >= 0 && live ? keep * (dt_exp2(e) / sum) : 0.f;
     if (!(v == 0.f)) h += v * (e - lg);
     a[i] = v;
@@ -111,11 +111,11 @@ distill_teacher_planes_kernel(const IT* __restrict__ idx, const TT* __restrict__
         live |= !(a == -INFINITY);
       }
     }
-    const float ref = dt_ref(mx, c);
+    const float ref = dt_ref(mx);
     float sum = 0.f;
     for (int k = 0; k < K; ++k) {
       const long long j = (long long)idx[base + k * S];
-      if (j >= 0 && j < V) sum += dt_exp2(__builtin_fmaf(ld1(top + base + k * S), c, -ref));
+      if (j >= 0 && j < V) sum += dt_term(ld1(top + base + k * S), ref, c);
     }
     const float r = live && rest ? rest[row] : 0.f;
     const float keep = 1.f - r, lg = log2f(sum) - log2f(keep);
@@ -126,7 +126,7 @@ distill_teacher_planes_kernel(const IT* __restrict__ idx, const TT* __restrict__
       float v = 0.f;
       if (live && j >= 0 && j < V) {
         mine = (int)j;
-        const float e = __builtin_fmaf(ld1(top + base + k * S), c, -ref);
+        const float e = (ld1(top + base + k * S) - ref) * c;
         v = keep * (dt_exp2(e) / sum);
         if (!(v == 0.f)) h += v * (e - lg);
         for (int q = 0; q < k; ++q)  // listed before: its mass joins the first entry
@@ -192,7 +192,7 @@ ACC_DEV void dtp_gradient(const T* zr, T* dr, long S, int V, int K, const int* i
       if (j0 + u >= V) continue;
       const float pj = TAB ? tab[(j0 + u) * 256] : -1.f;
       const bool free = pj == -1.f;
-      const float e = dt_exp2(__builtin_fmaf(v[u], c, free ? -st.x : -st.z));
+      const float e = dt_term(v[u], free ? st.x : st.z, c);
       st1(dr + (long)(j0 + u) * S, free ? e * cu : gs * (e * st.w - pj));
     }
   }
@@ -200,8 +200,7 @@ ACC_DEV void dtp_gradient(const T* zr, T* dr, long S, int V, int K, const int* i
   for (int k = 0; k < K; ++k) {
     const int j = id[k * S];
     if (j >= 0)
-      st1(dr + (long)j * S, gs * (dt_exp2(__builtin_fmaf(ld1(zr + (long)j * S), c, -st.z)) * st.w -
-                                  p[k * S]));
+      st1(dr + (long)j * S, gs * (dt_term(ld1(zr + (long)j * S), st.z, c) * st.w - p[k * S]));
   }
 }
 template <typename T>
@@ -260,9 +259,9 @@ distill_planes_fwd_kernel(const DtArgs a, const DtScale g) {
           s *= dt_rescale(m, mv, c);
           m = mv;
         }
-        const float ref = dt_ref(m, c);
+        const float ref = dt_ref(m);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) s += dt_exp2(__builtin_fmaf(v[u], c, -ref));
+        for (int u = 0; u < 4; ++u) s += dt_term(v[u], ref, c);
       }
       const float mr = m, sr = s;
       if (REST)
@@ -277,9 +276,9 @@ distill_planes_fwd_kernel(const DtArgs a, const DtScale g) {
         const int j = a.id[kb + k * S];
         const float pk = a.p[kb + k * S];
         if (j >= 0 && !(pk == 0.f))
-          dot += pk * (__builtin_fmaf(ld1(zr + (long)j * S), c, -o.M) - o.log2S);
+          dot += pk * dt_log2q(ld1(zr + (long)j * S), o, c);
       }
-      if (REST && !(r == 0.f)) dot += r * ((dt_ref(mr, c) - o.M) + log2f(sr) - o.log2S);
+      if (REST && !(r == 0.f)) dot += r * dt_log2q_rest(mr, sr, o, c);
       a.state[row] = o.state;
       loss = a.scale * (te.x - dot);
       if (dr)

@@ -143,11 +143,11 @@ ACC_DEV void dt_stream(const T* z, int off, int V, int q0, int q1, const int* id
         s *= dt_rescale(m, mv, c);
         m = mv;
       }
-      const float ref = dt_ref(m, c);
+      const float ref = dt_ref(m);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += dt_exp2(__builtin_fmaf(get(u, e), c, -ref));
+        for (int e = 0; e < N; ++e) s += dt_term(get(u, e), ref, c);
     };
     for (int q = qc + t; q < qe; q += NT * U) {
       if (run.whole(__builtin_amdgcn_readfirstlane(q), NT, U, qe)) {
@@ -202,11 +202,10 @@ ACC_DEV float4 dt_finish_row(F zk, const int* id, const float* p, int K, float m
   float dot = 0.f;
   for (int k = lane; k < K; k += 64) {
     const float pk = p[k];
-    if (id[k] >= 0 && !(pk == 0.f))
-      dot += pk * (__builtin_fmaf(zk(k), c, -o.M) - o.log2S);
+    if (id[k] >= 0 && !(pk == 0.f)) dot += pk * dt_log2q(zk(k), o, c);
   }
   dot = dt_wave_sum(dot);
-  if (has_rest && !(rest == 0.f)) dot += rest * ((dt_ref(mr, c) - o.M) + log2f(sr) - o.log2S);
+  if (has_rest && !(rest == 0.f)) dot += rest * dt_log2q_rest(mr, sr, o, c);
   if (lane == 0) {
     const float loss = scale * (h - dot);
     *state = o.state;
@@ -228,7 +227,7 @@ ACC_DEV void dt_empty_row(int lane, float4* state, float* rowloss, double* part)
 template <typename T>
 ACC_DEV void dt_put_listed(const T* zr, T* dr, int j, float p, const float4& st, float c,
                            float gs) {
-  st1(dr + j, gs * (dt_exp2(__builtin_fmaf(ld1(zr + j), c, -st.z)) * st.w - p));
+  st1(dr + j, gs * (dt_term(ld1(zr + j), st.z, c) * st.w - p));
 }
 
 // Gradient of vectors [q0, q1) of a row by threads t of NT: every class as not listed, then,
@@ -253,7 +252,7 @@ ACC_DEV void dt_gradient(const T* zr, T* dr, int off, int V, int q0, int q1, con
       if (q + u * NT >= q1) continue;
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        v[u][e] = live ? dt_exp2(__builtin_fmaf(v[u][e], c, -st.x)) * cu : 0.f;
+        v[u][e] = live ? dt_term(v[u][e], st.x, c) * cu : 0.f;
       dt_put<T, STREAM>(dr, off, V, q + u * NT, 0u, v[u]);
     }
   }
@@ -331,13 +330,13 @@ distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, v[u][e]);
       m = dt_wave_max(m);
-      const float ref = dt_ref(m, a.c);
+      const float ref = dt_ref(m);
       float s = 0.f;
 #pragma unroll
       for (int u = 0; u < NQ; ++u)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          v[u][e] = dt_exp2(__builtin_fmaf(v[u][e], a.c, -ref));
+          v[u][e] = dt_term(v[u][e], ref, a.c);
           s += v[u][e];
         }
       s = dt_wave_sum(s);
@@ -457,7 +456,7 @@ distill_rows_fused_kernel(const DtArgs a, const DtScale g) {
         float v[N];
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          v[e] = dt_exp2(__builtin_fmaf(dt_get<T>(w[u], e), a.c, -st.x)) * cu;
+          v[e] = dt_term(dt_get<T>(w[u], e), st.x, a.c) * cu;
         if (plain) DtVec<T>::template st<STREAM>(dr + (q + u * NT) * N - off, v);
         else dt_put<T, STREAM>(dr, off, V, q + u * NT, bits[u], v);
       }
@@ -469,7 +468,7 @@ distill_rows_fused_kernel(const DtArgs a, const DtScale g) {
       float v[N];
       dt_load(zr, off, V, q + u * NT, v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = dt_exp2(__builtin_fmaf(v[e], a.c, -st.x)) * cu;
+      for (int e = 0; e < N; ++e) v[e] = dt_term(v[e], st.x, a.c) * cu;
       dt_put<T, STREAM>(dr, off, V, q + u * NT, dt_mark(mark, q + u * NT), v);
     }
   }
