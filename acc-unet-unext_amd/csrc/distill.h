@@ -2,10 +2,11 @@
 //
 // Row i: student logits z[0..V), the teacher's entries (idx_k, t_k), k < K, an optional
 // mass `rest` of the teacher outside them, temperature T.
-//   p_k   = (1 - rest) * softmax(t / T)_k over the entries with 0 <= idx_k < V
+//   p_k   = (1 - rest) * softmax(t / T)_k over the entries with 0 <= idx_k < V; entries of one
+//           class are one entry with their sum from here on
 //   q     = softmax(z / T) over all V classes, q_rest = sum of q over classes not listed
 //   loss  = T^2 * [ sum_k p_k (log p_k - log q_idx_k) + rest (log rest - log q_rest) ]
-//   dloss/dz_j = T * (q_j - p_j)                  listed (p_j: the sum over its entries)
+//   dloss/dz_j = T * (q_j - p_j)                  listed
 //              = T * (q_j - rest * q_j / q_rest)  not listed
 // A row without a valid entry (or whose valid t are all -inf) has loss 0 and gradient 0
 // and is not counted by the mean.
@@ -37,6 +38,8 @@ ACC_DEV float dt_rescale(float m, float M, float c) { return m == M ? 1.f : dt_e
 ACC_DEV float dt_ref(float m) { return m == -INFINITY ? 0.f : m; }
 // 2^((z - ref) * c)
 ACC_DEV float dt_term(float z, float ref, float c) { return dt_exp2((z - ref) * c); }
+// p log2 p
+ACC_DEV float dt_plogp(float p) { return p == 0.f ? 0.f : p * log2f(p); }
 // (m, s) joined with (m2, s2)
 ACC_DEV void dt_join(float& m, float& s, float m2, float s2, float c) {
   const float M = fmaxf(m, m2);

@@ -52,21 +52,15 @@ distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ t
     if (my[i] >= 0) sum += dt_term(a[i], ref, c);
   sum = dt_wave_sum(sum);
   const float r = in && live && rest ? rest[row] : 0.f;
-  const float keep = 1.f - r, lg = log2f(sum) - log2f(keep);
-  float h = 0.f;
+  const float keep = 1.f - r;
 #pragma unroll
   for (int i = 0; i < DT_MAX_K / 64; ++i) {
     const int k = i * 64 + lane;
     if (i >= NI || k >= K) continue;
-    const float e = (a[i] - ref) * c;
-    const float v = my[i] >= 0 && live ? keep * (dt_exp2(e) / sum) : 0.f;
-    if (!(v == 0.f)) h += v * (e - lg);
-    a[i] = v;
     sid[wave][k] = my[i];
-    sp[wave][k] = v;
+    sp[wave][k] = my[i] >= 0 && live ? keep * (dt_term(a[i], ref, c) / sum) : 0.f;
   }
-  h = dt_wave_sum(h);
-  if (r != 0.f) h += r * log2f(r);
+  float h = 0.f;  // of the classes' masses, not of their entries'
   dt_wave_lds();
 #pragma unroll
   for (int i = 0; i < DT_MAX_K / 64; ++i) {
@@ -81,7 +75,9 @@ distill_teacher_rows_kernel(const IT* __restrict__ idx, const TT* __restrict__ t
       }
     id[row * K + k] = first ? my[i] : -1;
     p[row * K + k] = v;
+    if (first) h += dt_plogp(v);
   }
+  h = dt_wave_sum(h) + dt_plogp(r);
   if (lane == 0) {
     if (in) tea[row] = make_float2(h, live ? 1.f : 0.f);
     alive[wave] = in && live ? 1 : 0;
@@ -118,22 +114,23 @@ distill_teacher_planes_kernel(const IT* __restrict__ idx, const TT* __restrict__
       if (j >= 0 && j < V) sum += dt_term(ld1(top + base + k * S), ref, c);
     }
     const float r = live && rest ? rest[row] : 0.f;
-    const float keep = 1.f - r, lg = log2f(sum) - log2f(keep);
-    float h = r != 0.f ? r * log2f(r) : 0.f;
+    const float keep = 1.f - r;
+    float h = dt_plogp(r);
     for (int k = 0; k < K; ++k) {
       const long long j = (long long)idx[base + k * S];
       int mine = -1;
       float v = 0.f;
       if (live && j >= 0 && j < V) {
         mine = (int)j;
-        const float e = (ld1(top + base + k * S) - ref) * c;
-        v = keep * (dt_exp2(e) / sum);
-        if (!(v == 0.f)) h += v * (e - lg);
+        v = keep * (dt_term(ld1(top + base + k * S), ref, c) / sum);
         for (int q = 0; q < k; ++q)  // listed before: its mass joins the first entry
           if (mine >= 0 && id[base + q * S] == mine) {
-            p[base + q * S] += v;
+            const float was = p[base + q * S];
+            p[base + q * S] = was + v;
+            h += dt_plogp(was + v) - dt_plogp(was);
             mine = -1;
           }
+        if (mine >= 0) h += dt_plogp(v);
       }
       id[base + k * S] = mine;
       p[base + k * S] = mine >= 0 ? v : 0.f;

@@ -24,9 +24,21 @@ GLOO_ON_ONE_GPU = ("test_world4_buckets_and_wire_against_fp64_mean",
                    "test_bench_gpus4_gloo_reports_four_ranks")
 
 
+# test_distill.py::test_hard_rows expects a wrong loss of its row 4, which lists one class many
+# times: its reference adds p log p of each entry, where the distribution has the class's whole
+# mass. Two equal entries of one class make -T^2 log 2 of two equal distributions, and no
+# Kullback-Leibler divergence is negative. test_distill_values.py has the same rows against
+# the whole mass.
+WRONG_VALUE = {"test_distill.py": ("test_hard_rows",)}
+
+
 def pytest_collection_modifyitems(config, items):
     import pytest
     for item in items:
+        if item.originalname in WRONG_VALUE.get(item.path.name, ()):
+            item.add_marker(pytest.mark.xfail(
+                strict=True, raises=AssertionError,
+                reason="its reference counts a repeated class by entries"))
         if item.name in GLOO_ON_ONE_GPU:
             item.add_marker(pytest.mark.skip(
                 reason="stopped after 180 s of silence: device tensors over gloo between more "

@@ -1,5 +1,6 @@
 """Distillation (accunet/distill.py): logits far from zero or masked with the type's lowest
-value, against the definition in 64 bits on distributions over all classes.
+value, and classes listed more than once, against the definition in 64 bits on distributions
+over all classes.
 
 Tolerance, u = 2^-24, e the exponent (z - m) * log2(e) / T of a softmax term: the difference,
 the factor and the product round once each, so 2^e is off by 3 u |e| ln 2 + 2 u (exp2); the
@@ -13,7 +14,7 @@ import math
 
 import pytest
 import torch
-from test_distill import NEG, U, _close, _fn, _make
+from test_distill import NEG, U, _close, _fn, _hard, _make
 
 
 def _exact(z, idx, top, rest, T):
@@ -51,7 +52,7 @@ def _exact(z, idx, top, rest, T):
     has = ok & (top > NEG)
     spread = (torch.where(has, top, torch.full_like(top, NEG)).amax(1)
               - torch.where(has, top, torch.full_like(top, math.inf)).amin(1))
-    D = (torch.maximum(hi - lo, spread) / T * 1.4427).clamp(max=150.0)
+    D = (torch.maximum(hi - lo, spread) / T * 1.4427).clamp(min=0.0, max=150.0)
     k = (9 * D + 100 + idx.shape[1]) * U
     z0 = torch.zeros((), dtype=torch.float64)
     loss, mag = torch.where(live, loss, z0) * T * T, torch.where(live, mag, z0) * T * T
@@ -121,3 +122,58 @@ def test_classes_masked_with_the_lowest_value(R, V, K, planes, T, dtype):
             free = torch.ones(R, V, dtype=torch.bool).scatter_(1, idx, False)
             r[~(free & (z > lowest)).any(1) & (torch.arange(R) != 2)] = 0.0
         _compare(z, idx, top, r, T, planes)
+
+
+REPEATED = [(8, 7, 3, None), (9, 40, 6, None), (7, 257, 200, None), (6, 5003, 256, None),
+            (260, 2500, 9, None), (12, 12, 4, (2, 6)), (10, 150, 70, (2, 5))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V,K,planes", REPEATED)
+def test_repeated_entries_add_up(R, V, K, planes, dtype):
+    """p log p is taken of a class's whole mass, however many entries it is split over."""
+    for i, rest in enumerate((False, True)):
+        z, _, top, r = _make(R, V, 1, dtype, rest, seed=50 + i)
+        g = torch.Generator().manual_seed(60 + i)
+        idx = torch.randint(0, max(2, min(V, K // 2)), (R, K), generator=g)
+        top = (2 * torch.randn(R, K, generator=g)).to(dtype)
+        idx[0] = V - 1                   # one class
+        idx[1, ::2] = -1                 # padding between the entries
+        top[2, :K // 2] = NEG            # entries of no mass beside others of their class
+        idx[3], top[3, 1:] = 1, NEG      # a class's first entry has all its mass
+        idx[4], top[4, :-1] = 1, NEG     # its last one
+        top[5] = torch.linspace(-60, 0, K).to(dtype)  # masses of very different size
+        _compare(z, idx, top, r, 1.7, planes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("V", [30, 900])
+@pytest.mark.parametrize("K", [2, 3, 65, 256])
+def test_a_certain_student_has_no_loss(K, V, planes):
+    """Equal entries of one class, of which the student is certain: the distributions are the
+    same, so loss and gradient are zero. K masses of 1 / K add up to 1 within K u, and
+    log2 1 is 0; the student's other classes have 2^-140 of its mass at most."""
+    z = torch.full((4, V, 3) if planes else (4, V), -100.0, device="cuda")
+    shape = (4, K, 3) if planes else (4, K)
+    z[:, 5] = 0.0
+    z.requires_grad_()
+    idx = torch.full(shape, 5, device="cuda")
+    loss = _fn()(z, idx, torch.zeros(shape, device="cuda"), temperature=1.0, reduction="sum", dim=1)
+    (dz,) = torch.autograd.grad(loss, z)
+    assert abs(float(loss.detach())) <= 12 * (2 * K + 4) * U and float(dz.abs().max()) <= (2 * K + 4) * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,K,planes", [(40, 6, None), (40, 6, (2, 7)), (3001, 70, None),
+                                        (1000, 70, (2, 7))])
+def test_hard_rows(V, K, dtype, planes):
+    """The rows of test_distill.py's _hard, among them one that lists a class many times."""
+    z, idx, top, r = _hard(V, K, dtype)
+    for rest in (r, None):
+        _compare(z, idx, top, rest, 1.7, planes)
+    z[7, idx[7, 0]] = 0.0  # every loss finite
+    for rest in (r, None):
+        _compare(z, idx, top, rest, 1.7, planes)
