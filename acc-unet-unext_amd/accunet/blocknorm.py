@@ -23,33 +23,58 @@ from ._lib import AccError
 KINDS = ("layer", "rms")
 
 
-def _forward(x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L, keep):
-    C = x.shape[-1]
+def _check(x, f, params, g):
+    """Types, devices and sizes; rows P, rows that share a gate L, channels C."""
+    kern._check(x, "blocknorm x", act=True)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
+        raise AccError(f"blocknorm: 1 to 8192 channels on the last axis, got {tuple(x.shape)}")
+    C = int(x.shape[-1])
     P = x.numel() // C
-    r = torch.empty_like(x) if f is not None else None
-    h = torch.empty_like(x) if want_h else None
-    stats = torch.empty(P, 4, dtype=torch.float32, device=x.device) if keep else None
-    kern.blocknorm_fwd(x, f, w1, b1, s, g, w2, b2, layer, eps, r, h, stats, P, L, C)
-    return r, h, stats
+    for name, t in (("f", f), ("gate", g)):
+        if t is not None and (t.dtype != x.dtype or t.get_device() != x.get_device()):
+            raise AccError(f"sandwich_norm {name}: {x.dtype} on {x.device} expected, got "
+                           f"{t.dtype} on {t.device}")
+    if f is not None and f.shape != x.shape:
+        raise AccError(f"sandwich_norm: f {tuple(f.shape)} and x {tuple(x.shape)} differ")
+    for name, t in params:
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != C
+                              or t.get_device() != x.get_device()):
+            raise AccError(f"{name}: float32 [{C}] on {x.device} expected, got {t.dtype} "
+                           f"{tuple(t.shape)} on {t.device}")
+    L = P
+    if g is not None:
+        shared = (x.shape[0],) + (1,) * (x.dim() - 2) + (C,) if x.dim() >= 2 else None
+        if g.shape == x.shape:
+            L = 1
+        elif tuple(g.shape) == shared:
+            L = P // x.shape[0] if P else 1
+        else:
+            raise AccError(f"sandwich_norm: gate {tuple(g.shape)} is neither x's shape "
+                           f"{tuple(x.shape)} nor one row per sample {shared}")
+    return P, L, C
 
 
 def _apply(*args):
-    """The formulas on checked arguments; the autograd node only where a gradient may flow."""
-    if torch.is_grad_enabled():
-        for t in args[:8]:
-            if t is not None and t.requires_grad:
-                return _BlockNormFn.apply(*args)
-    return _forward(*args, False)[:2]
+    """Every call goes through the autograd function, one without a backward (`keep`) too:
+    forward mode refuses it and a trace records it, where a launch of its own would pass both
+    by. Checks and sizes are its own, so a replayed trace has those of its inputs."""
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8])
+    return _BlockNormFn.apply(*args, keep)
 
 
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L):
-        r, h, stats = _forward(x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, L, True)
-        C = x.shape[-1]
-        ctx.save_for_backward(x, f, w1, b1, s, g, w2, stats)
-        ctx.cfg = (layer, x.numel() // C, L, C)
-        ctx.set_materialize_grads(False)
+    def forward(ctx, x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, keep):
+        P, L, C = _check(x, f, (("post_weight", w1), ("post_bias", b1), ("scale", s),
+                                ("pre_weight", w2), ("pre_bias", b2)), g)
+        r = torch.empty_like(x) if f is not None else None
+        h = torch.empty_like(x) if want_h else None
+        stats = torch.empty(P, 4, dtype=torch.float32, device=x.device) if keep else None
+        kern.blocknorm_fwd(x, f, w1, b1, s, g, w2, b2, layer, eps, r, h, stats, P, L, C)
+        if keep:
+            ctx.save_for_backward(x, f, w1, b1, s, g, w2, stats)
+            ctx.cfg = (layer, P, L, C)
+            ctx.set_materialize_grads(False)
         return r, h
 
     @staticmethod
@@ -68,30 +93,17 @@ class _BlockNormFn(torch.autograd.Function):
         kern.blocknorm_bwd(x, f, w1, b1, s, g, w2, layer, stats, dr, dh, dx, df, dg, dpar, P, L, C)
         par = [d if on else None for d, on in zip(dpar.unbind(0), ctx.needs_input_grad[2:5]
                                                   + ctx.needs_input_grad[6:8])]
-        return (dx, df, par[0], par[1], par[2], dg, par[3], par[4], None, None, None, None)
+        return (dx, df, par[0], par[1], par[2], dg, par[3], par[4]) + (None,) * 4
 
 
-def _param(t, C, name, x):
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != C or t.get_device() != x.get_device():
-        raise AccError(f"{name}: float32 [{C}] on {x.device} expected, got {t.dtype} "
-                       f"{tuple(t.shape)} on {t.device}")
-    return t.contiguous()
-
-
-def _act(t, name, x):
-    if t.dtype != x.dtype or t.get_device() != x.get_device():
-        raise AccError(f"{name}: {x.dtype} on {x.device} expected, got {t.dtype} on {t.device}")
-    return t.contiguous()
-
-
-def _check_x(x, kind):
+def _kind(kind):
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {KINDS}, got {kind!r}")
-    kern._check(x, "blocknorm x", act=True)
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
-        raise AccError(f"blocknorm: 1 to 8192 channels on the last axis, got {tuple(x.shape)}")
+    return kind == "layer"
+
+
+def _rows(*ts):
+    return [None if t is None else t.contiguous() for t in ts]
 
 
 def sandwich_norm(x, f, post_weight=None, post_bias=None, scale=None, gate=None,
@@ -101,37 +113,17 @@ def sandwich_norm(x, f, post_weight=None, post_bias=None, scale=None, gate=None,
     x, f: [..., C]. gate: None, x's shape, or x's shape with every axis but the first and
     the last 1 ([B, 1, ..., C], one row per sample). Weights and scale None mean 1, biases
     None mean 0."""
-    _check_x(x, kind)
-    C = x.shape[-1]
-    if f.shape != x.shape:
-        raise AccError(f"sandwich_norm: f {tuple(f.shape)} and x {tuple(x.shape)} differ")
+    layer = _kind(kind)
     if not pre and (pre_weight is not None or pre_bias is not None):
         raise ValueError("sandwich_norm: pre=False takes no pre_weight / pre_bias")
-    P = x.numel() // C
-    L = P
-    if gate is not None:
-        shared = (x.shape[0],) + (1,) * (x.dim() - 2) + (C,) if x.dim() >= 2 else None
-        if gate.shape == x.shape:
-            L = 1
-        elif tuple(gate.shape) == shared:
-            L = P // x.shape[0] if P else 1
-        else:
-            raise AccError(f"sandwich_norm: gate {tuple(gate.shape)} is neither x's shape "
-                           f"{tuple(x.shape)} nor one row per sample {shared}")
-        gate = _act(gate, "sandwich_norm gate", x)
-    return _apply(x.contiguous(), _act(f, "sandwich_norm f", x),
-                  _param(post_weight, C, "post_weight", x), _param(post_bias, C, "post_bias", x),
-                  _param(scale, C, "scale", x), gate, _param(pre_weight, C, "pre_weight", x),
-                  _param(pre_bias, C, "pre_bias", x), kind == "layer", float(eps), bool(pre), L)
+    return _apply(*_rows(x, f, post_weight, post_bias, scale, gate, pre_weight, pre_bias), layer,
+                  float(eps), bool(pre))
 
 
 def norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
     """norm(x) * weight + bias over the last axis: the norm before a model's first block."""
-    _check_x(x, kind)
-    C = x.shape[-1]
-    w, b = _param(weight, C, "weight", x), _param(bias, C, "bias", x)
-    return _apply(x.contiguous(), None, None, None, None, None, w, b, kind == "layer",
-                  float(eps), True, x.numel() // C)[1]
+    layer = _kind(kind)
+    return _apply(*_rows(x, None, None, None, None, None, weight, bias), layer, float(eps), True)[1]
 
 
 class SandwichNorm(nn.Module):

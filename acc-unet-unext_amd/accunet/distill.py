@@ -17,6 +17,8 @@ probability 0 (infinite loss where the teacher has mass there).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import kern
@@ -27,13 +29,33 @@ _PLANES_MAX_V = 1024
 _REDUCTIONS = ("none", "sum", "mean")
 
 
-def _forward(z, idx, top, rest, T, weight, reduction, B, S, V, K, dz):
-    n = B * S
-    none = reduction == 0
-    if n == 0:
-        return torch.zeros((0,) if none else (), dtype=torch.float32, device=z.device), None
-    loss = torch.empty((n,) if none else (), dtype=torch.float32, device=z.device)
-    return loss, kern.distill_fwd(z, idx, top, rest, loss, reduction, dz, B, S, V, K, T, weight)
+def _sizes(z, idx, top, rest, planes):
+    """Checks; B, S, V, K of the kernels (rows: B of them, S = 1)."""
+    kern._check(z, "topk_distill logits", act=True)
+    axis, shape = 1 if planes else z.dim() - 1, tuple(z.shape)
+    V, K = int(shape[axis]), (int(idx.shape[axis]) if idx.dim() == z.dim() else 0)
+    want, outer = shape[:axis] + (K,) + shape[axis + 1:], shape[:axis] + shape[axis + 1:]
+    if not 1 <= K <= MAX_K or tuple(idx.shape) != want or tuple(top.shape) != want:
+        raise AccError(f"topk_distill: top_idx {tuple(idx.shape)} and top_logits "
+                       f"{tuple(top.shape)} must have 1 to {MAX_K} entries in place of "
+                       f"the {V} classes of {shape}")
+    if not 1 <= V <= 1 << 30:
+        raise AccError(f"topk_distill: 1 to 2^30 classes, got {V}")
+    if idx.dtype not in (torch.int32, torch.int64):
+        raise AccError(f"topk_distill: int32 or int64 top_idx, got {idx.dtype}")
+    kern._check(top, "topk_distill top_logits", act=True)
+    if rest is not None:
+        kern._check(rest, "topk_distill rest")
+        if tuple(rest.shape) != outer:
+            raise AccError(f"topk_distill: rest {tuple(rest.shape)}, expected {outer}")
+    for name, t in (("top_idx", idx), ("top_logits", top), ("rest", rest)):
+        if t is not None and t.device != z.device:
+            raise AccError(f"topk_distill: {name} on {t.device}, logits on {z.device}")
+    n = 1
+    for s in outer:
+        n *= int(s)
+    B = int(shape[0]) if planes else n
+    return B, (n // B if B else 0) if planes else 1, V, K, outer
 
 
 class _DistillFn(torch.autograd.Function):
@@ -41,16 +63,28 @@ class _DistillFn(torch.autograd.Function):
     (sum and mean), and the backward hands that tensor out, once: its kernel rewrites it only
     for another upstream gradient. A further backward of the same graph computes it anew, and
     so does a backward in another graph capture than the forward's: replayed by itself, it
-    would hand out what the consumers of the last replay left in that tensor."""
+    would hand out what the consumers of the last replay left in that tensor.
+
+    Every call goes through here, one without a backward (`grad`) too: forward mode refuses it
+    and a trace records it, where a launch of its own would pass both by. Checks and sizes are
+    its own, so a replayed trace has those of its inputs."""
 
     @staticmethod
-    def forward(ctx, z, idx, top, rest, T, weight, reduction, B, S, V, K):
-        fuse = reduction != 0 and B * S > 0 and kern.distill_fused(B, S, V, kern._dt(z))
-        ctx.dz = torch.empty_like(z) if fuse else None
-        loss, save = _forward(z, idx, top, rest, T, weight, reduction, B, S, V, K, ctx.dz)
-        ctx.capture = kern.capture_id(z)
-        ctx.save_for_backward(z, save)
-        ctx.cfg = (reduction, B, S, V, K, T, weight)
+    def forward(ctx, z, idx, top, rest, T, weight, reduction, planes, grad):
+        B, S, V, K, outer = _sizes(z, idx, top, rest, planes)
+        new = torch.empty if B * S else torch.zeros
+        loss = new(outer if reduction == 0 else (), dtype=torch.float32, device=z.device)
+        if z.data_ptr() % 16:
+            z = z.clone()
+        dz = save = None
+        if grad and reduction != 0 and B * S and kern.distill_fused(B, S, V, kern._dt(z)):
+            dz = torch.empty_like(z)
+        if B * S:
+            save = kern.distill_fwd(z, idx, top, rest, loss, reduction, dz, B, S, V, K, T, weight)
+        if grad:
+            ctx.dz, ctx.capture = dz, kern.capture_id(z)
+            ctx.save_for_backward(z, save)
+            ctx.cfg = (reduction, B, S, V, K, T, weight)
         return loss
 
     @staticmethod
@@ -64,7 +98,7 @@ class _DistillFn(torch.autograd.Function):
         if save is not None:
             reduction, B, S, V, K, T, weight = ctx.cfg
             kern.distill_bwd(z, save, up.contiguous(), reduction, held, dz, B, S, V, K, T, weight)
-        return (dz,) + (None,) * 10
+        return (dz,) + (None,) * 8
 
 
 def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight=1.0,
@@ -84,52 +118,21 @@ def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight
     temperature, weight = float(temperature), float(weight)
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    kern._check(logits, "topk_distill logits", act=True)
     nd = logits.dim()
     axis = dim + nd if dim < 0 else dim
     if nd < 1 or axis not in (nd - 1, 1) or not 0 <= axis < nd:
         raise AccError(f"topk_distill: the classes lie on the last axis or on axis 1, got "
                        f"dim={dim} of {tuple(logits.shape)}")
-    shape = list(logits.shape)
-    V, K = shape[axis], (top_idx.shape[axis] if top_idx.dim() == nd else 0)
-    want = shape[:axis] + [K] + shape[axis + 1:]
-    outer = shape[:axis] + shape[axis + 1:]
-    if not 1 <= K <= MAX_K or list(top_idx.shape) != want or list(top_logits.shape) != want:
-        raise AccError(f"topk_distill: top_idx {tuple(top_idx.shape)} and top_logits "
-                       f"{tuple(top_logits.shape)} must have 1 to {MAX_K} entries in place of "
-                       f"the {V} classes of {tuple(shape)}")
-    if not 1 <= V <= 1 << 30:
-        raise AccError(f"topk_distill: 1 to 2^30 classes, got {V}")
-    if top_idx.dtype not in (torch.int32, torch.int64):
-        raise AccError(f"topk_distill: int32 or int64 top_idx, got {top_idx.dtype}")
-    kern._check(top_logits, "topk_distill top_logits", act=True)
-    if rest is not None:
-        kern._check(rest, "topk_distill rest")
-        if list(rest.shape) != outer:
-            raise AccError(f"topk_distill: rest {tuple(rest.shape)}, expected {tuple(outer)}")
     for name, t in (("top_idx", top_idx), ("top_logits", top_logits), ("rest", rest)):
-        if t is not None and t.device != logits.device:
-            raise AccError(f"topk_distill: {name} on {t.device}, logits on {logits.device}")
         if t is not None and t.requires_grad:
             raise ValueError(f"topk_distill: no gradient flows to {name}; detach it")
-    S = 1
-    for s in shape[axis + 1:]:
-        S *= s
-    planes = axis != nd - 1 and S > 1
-    if planes and V > _PLANES_MAX_V:
-        logits, top_idx, top_logits = (t.movedim(axis, -1) for t in (logits, top_idx, top_logits))
+    args = (logits, top_idx, top_logits)
+    planes = axis != nd - 1
+    if planes and (logits.shape[1] > _PLANES_MAX_V or math.prod(logits.shape[2:]) <= 1):
+        # too many classes, or one pixel a sample (no copy then)
+        args = [t.movedim(axis, -1) if t.dim() == nd else t for t in args]
         planes = False
-    B = 1
-    for s in (shape[:axis] if planes else outer):
-        B *= s
-    z = logits.contiguous()
-    if z.data_ptr() % 16:
-        z = z.clone()
-    args = (z, top_idx.contiguous(), top_logits.contiguous(),
-            rest.contiguous() if rest is not None else None, temperature, weight,
-            _REDUCTIONS.index(reduction), B, S if planes else 1, V, K)
-    if z.requires_grad and torch.is_grad_enabled():
-        loss = _DistillFn.apply(*args)
-    else:
-        loss = _forward(*args, None)[0]
-    return loss.view(outer) if reduction == "none" else loss
+    return _DistillFn.apply(*(t.contiguous() for t in args),
+                            rest.contiguous() if rest is not None else None, temperature, weight,
+                            _REDUCTIONS.index(reduction), planes,
+                            torch.is_grad_enabled() and logits.requires_grad)

@@ -93,27 +93,54 @@ def quantize(x, square=False, transposed=False):
     return Fp8Blocks(q, s, R, C, square, t)
 
 
-def _forward(x, weight, bias, wq, N, need_w=False, need_wt=False):
-    """y, and what the gradients need: the transposed x and (of a float weight) weight."""
-    K = x.shape[-1]
-    M = x.numel() // K
-    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    if M == 0:
-        return y, None
-    q, s = (None, None) if wq is None else (wq.q, wq.s)
-    return y, kern.fp8_linear_fwd(x, weight, q, s, bias, y, need_w, need_wt, M, N, K)
+def _sizes(x, weight, bias, wq, need_x):
+    """Checks; tokens M, output and input features N, K."""
+    kern._check(x, "fp8.linear x", act=True)
+    w = weight
+    if wq is None:
+        kern._check(weight, "fp8.linear weight")
+        if weight.dim() != 2:
+            raise AccError(f"fp8.linear: weight [N, K] expected, got {tuple(weight.shape)}")
+    else:
+        w = wq
+        if not wq.square:
+            raise AccError("fp8.linear: a frozen weight needs blocks of 128 x 128 "
+                           "(quantize(w, square=True))")
+        if need_x and wq.t is None:
+            raise AccError("fp8.linear: the gradient of x needs the transposed weight "
+                           "(quantize(w, square=True, transposed=True))")
+    N, K = (int(n) for n in w.shape)
+    if x.dim() < 1 or x.shape[-1] != K or not (1 <= N <= _MAX_DIM and 1 <= K <= _MAX_DIM):
+        raise AccError(f"fp8.linear: x {tuple(x.shape)} and weight {(N, K)} do not match")
+    if w.device != x.device:
+        raise AccError(f"fp8.linear: weight on {w.device}, x on {x.device}")
+    if bias is not None:
+        kern._check(bias, "fp8.linear bias")
+        if tuple(bias.shape) != (N,) or bias.device != x.device:
+            raise AccError(f"fp8.linear: bias {tuple(bias.shape)} on {bias.device}, expected "
+                           f"{(N,)} on {x.device}")
+    return x.numel() // K, N, K
 
 
 class _LinearFn(torch.autograd.Function):
+    """Every call goes through here, one without a backward (`grad`) too: forward mode refuses
+    it and a trace records it, where a launch of its own would pass both by. Checks and sizes
+    are its own, so a replayed trace has those of its inputs."""
+
     @staticmethod
-    def forward(ctx, x, weight, bias, wq, N):
-        need_x, need_w = ctx.needs_input_grad[:2]
+    def forward(ctx, x, weight, bias, wq, grad):
+        need_x, need_w = (grad and need for need in ctx.needs_input_grad[:2])
+        M, N, K = _sizes(x, weight, bias, wq, need_x)
         need_wt = need_x and weight is not None
-        y, save = _forward(x, weight, bias, wq, N, need_w, need_wt)
-        t = wq.t if need_x and wq is not None else None
-        ctx.save_for_backward(save, *((t.q, t.s) if t is not None else (None, None)))
-        K = x.shape[-1]
-        ctx.cfg = (x.numel() // K, N, K, x.shape, x.dtype, need_w, need_wt)
+        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        save = None
+        if M:
+            q, s = (None, None) if wq is None else (wq.q, wq.s)
+            save = kern.fp8_linear_fwd(x, weight, q, s, bias, y, need_w, need_wt, M, N, K)
+        if grad:
+            t = wq.t if need_x and wq is not None else None
+            ctx.save_for_backward(save, *((t.q, t.s) if t is not None else (None, None)))
+            ctx.cfg = (M, N, K, x.shape, x.dtype, need_w, need_wt)
         return y
 
     @staticmethod
@@ -134,41 +161,12 @@ class _LinearFn(torch.autograd.Function):
 def linear(x, weight, bias=None):
     """The layer of the module docstring on x [..., K]: weight float32 [N, K], or a frozen
     one as quantize(w, square=True) left it; bias float32 [N] or None. Returns x's type."""
-    kern._check(x, "fp8.linear x", act=True)
-    frozen = isinstance(weight, Fp8Blocks)
-    if not frozen:
-        kern._check(weight, "fp8.linear weight")
-        if weight.dim() != 2:
-            raise AccError(f"fp8.linear: weight [N, K] expected, got {tuple(weight.shape)}")
-    N, K = weight.shape
-    if x.dim() < 1 or x.shape[-1] != K or not (1 <= N <= _MAX_DIM and 1 <= K <= _MAX_DIM):
-        raise AccError(f"fp8.linear: x {tuple(x.shape)} and weight {(N, K)} do not match")
-    if weight.device != x.device:
-        raise AccError(f"fp8.linear: weight on {weight.device}, x on {x.device}")
-    if bias is not None:
-        kern._check(bias, "fp8.linear bias")
-        if tuple(bias.shape) != (N,) or bias.device != x.device:
-            raise AccError(f"fp8.linear: bias {tuple(bias.shape)} on {bias.device}, expected "
-                           f"{(N,)} on {x.device}")
-        bias = bias.contiguous()
-    grad = torch.is_grad_enabled() and (
-        x.requires_grad or (not frozen and weight.requires_grad)
-        or (bias is not None and bias.requires_grad))
-    x = x.contiguous()
-    wq = None
-    if frozen:
-        if not weight.square:
-            raise AccError("fp8.linear: a frozen weight needs blocks of 128 x 128 "
-                           "(quantize(w, square=True))")
-        if grad and x.requires_grad and weight.t is None:
-            raise AccError("fp8.linear: the gradient of x needs the transposed weight "
-                           "(quantize(w, square=True, transposed=True))")
-        wq, weight = weight, None
-    else:
-        weight = weight.contiguous()
-    if not grad:
-        return _forward(x, weight, bias, wq, N)[0]
-    return _LinearFn.apply(x, weight, bias, wq, N)
+    wq = weight if isinstance(weight, Fp8Blocks) else None
+    weight = None if wq is not None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                           for t in (x, weight, bias))
+    return _LinearFn.apply(x.contiguous(), weight, bias, wq, grad)
 
 
 class Linear(nn.Linear):
