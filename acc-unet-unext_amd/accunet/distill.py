@@ -26,6 +26,7 @@ from ._lib import AccError
 
 MAX_K = 256
 _PLANES_MAX_V = 1024
+_MIN_T = 2.0 ** -60  # T^2 and 1 / T are normal float32 numbers
 _REDUCTIONS = ("none", "sum", "mean")
 
 
@@ -109,6 +110,7 @@ def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight
     int64) and top_logits (float32 or bfloat16): the same shape with K <= 256 entries in
     place of the V classes. rest: float32, the shape without that axis, in [0, 1].
     reduction: "mean" over the rows that have an entry, "sum", or "none" (one loss a row).
+    temperature: 2^-60 to 2^60.
     `weight` multiplies the loss (inside: a factor applied to the result, 0.5 * loss, costs the
     backward another pass over the logits). Non-contiguous inputs are copied, and so are more than
     1024 classes on dim=1. At most 2^26 - 4 rows with the classes last, 2^24 - 1 above 2032
@@ -116,8 +118,8 @@ def topk_distill(logits, top_idx, top_logits, rest=None, temperature=1.0, weight
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     temperature, weight = float(temperature), float(weight)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not _MIN_T <= temperature <= 1 / _MIN_T:
+        raise ValueError(f"temperature must lie between 2^-60 and 2^60, got {temperature}")
     nd = logits.dim()
     axis = dim + nd if dim < 0 else dim
     if nd < 1 or axis not in (nd - 1, 1) or not 0 <= axis < nd:

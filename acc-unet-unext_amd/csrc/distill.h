@@ -24,6 +24,9 @@
 
 #define DT_MAX_K 256
 #define DT_MAX_V (1 << 30)
+// T^2 and log2(e) / T are normal fp32 numbers
+#define DT_MIN_T 0x1p-60f
+#define DT_MAX_T 0x1p60f
 #define DT_LN2 0.69314718055994531f
 #define DT_LOG2E 1.4426950408889634
 

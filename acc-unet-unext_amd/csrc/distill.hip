@@ -379,7 +379,7 @@ static int dt_check(long B, long S, int V, int K, float T) {
     return ACC_EBADSHAPE;
   if (dt_planes(S) && V > DTP_MAX_V) return ACC_EBADSHAPE;
   if (!dt_planes(S) && B > (V <= DTR_WAVE_V ? DTR_WAVE_ROWS : DTR_LONG_ROWS)) return ACC_EBADSHAPE;
-  return T > 0.f && T < INFINITY ? ACC_OK : ACC_EBADARG;
+  return T >= DT_MIN_T && T <= DT_MAX_T ? ACC_OK : ACC_EBADARG;
 }
 static DtArgs dt_args(long B, long S, int V, int K, float T, float weight) {
   DtArgs a = {};

@@ -518,7 +518,7 @@ int accunet_blocknorm_bwd(const void* x, const void* f, const float* w1, const f
  * "rows" z [R][V], or "planes" z [B][V][S] (classes on the channel axis; V <= 1024). The
  * teacher's K <= 256 entries a row: idx (int32, or int64 with idx64), top (storage top_dt),
  * [R][K] or [B][K][S]; an index outside [0, V) is padding. rest (fp32, one a row, or NULL):
- * the teacher's mass outside its entries. T > 0 the temperature, weight a factor of the loss.
+ * the teacher's mass outside its entries. T the temperature, 2^-60 to 2^60, weight a factor of the loss.
  *   p = (1 - rest) softmax(top / T), q = softmax(z / T)
  *   loss = weight T^2 [sum p (log p - log q) + rest (log rest - log q(not listed))]
  * A row without a valid entry has loss 0 and gradient 0.

@@ -14,6 +14,8 @@ import math
 
 import pytest
 import torch
+
+from accunet import _lib
 from test_distill import NEG, U, _close, _fn, _hard, _make
 
 
@@ -177,3 +179,26 @@ def test_hard_rows(V, K, dtype, planes):
     z[7, idx[7, 0]] = 0.0  # every loss finite
     for rest in (r, None):
         _compare(z, idx, top, rest, 1.7, planes)
+
+
+def test_temperatures_whose_square_leaves_fp32_are_refused():
+    """The loss is multiplied by T^2, its exponents by log2(e) / T: beyond 2^-60 and 2^60 one of
+    them overflowed or became zero, and with it the loss (NaN, or zero for a positive one)."""
+    z, i, t = torch.zeros(2, 5), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    for bad in (1e-45, 1e-39, 2.0 ** -61, 2.0 ** 61, 1e30, 1e39):
+        with pytest.raises(ValueError):
+            _fn()(z, i, t, temperature=bad)
+    lib = _lib.load()
+    n, m = lib.accunet_distill_save_bytes(2, 1, 5, 3), lib.accunet_distill_ws_bytes(2, 1, 5, 3, 0)
+    for bad in (1e-39, 2.0 ** -61, 2.0 ** 61, 1e30):
+        assert lib.accunet_distill_fwd(16, 16, 1, 16, 0, None, 16, 2, None, 16, n, 16, m, 2, 1, 5, 3,
+                                       bad, 1.0, 0, None) == -2
+        assert lib.accunet_distill_bwd(16, 16, n, 16, 2, 0, 16, 2, 1, 5, 3, bad, 1.0, 0, None) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2.0 ** -60, 2.0 ** -20, 2.0 ** 20, 2.0 ** 60])
+def test_extreme_temperatures(T):
+    """Logits of the size of T, so that the distributions are ordinary ones."""
+    z, idx, top, r = _make(5, 300, 6, torch.float32, True, seed=70)
+    _compare(z * T, idx, top * T, r, T)
