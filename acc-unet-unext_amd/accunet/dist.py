@@ -49,12 +49,37 @@ def local_device() -> int:
     return int(os.environ.get("LOCAL_RANK", "0")) % max(n, 1)
 
 
+# gloo gets CPU tensors only: its collectives on device tensors have hung where several ranks
+# share a GPU. Device tensors go through host memory then, by synchronous copies.
+def _through_host(t, group):
+    return t.is_cuda and dist.get_backend(group) != "nccl"
+
+
+def all_reduce(t: torch.Tensor, group=None, async_op: bool = False):
+    """In-place sum over ranks; returns the work to wait for, or None where it is done."""
+    if not _through_host(t, group):
+        return dist.all_reduce(t, op=dist.ReduceOp.SUM, group=group, async_op=async_op)
+    h = t.cpu()
+    dist.all_reduce(h, op=dist.ReduceOp.SUM, group=group)
+    t.copy_(h)
+    return None
+
+
+def broadcast(t: torch.Tensor, src: int, group=None):
+    if not _through_host(t, group):
+        dist.broadcast(t, src, group=group)
+        return
+    h = t.cpu()
+    dist.broadcast(h, src, group=group)
+    t.copy_(h)
+
+
 def all_reduce_mean(t: torch.Tensor, group=None):
     """In-place mean over ranks: RCCL's AVG, or SUM / world on backends without AVG."""
     if dist.get_backend(group) == "nccl":
         dist.all_reduce(t, op=dist.ReduceOp.AVG, group=group)
     else:
-        dist.all_reduce(t, op=dist.ReduceOp.SUM, group=group)
+        all_reduce(t, group=group)
         t.div_(dist.get_world_size(group))
 
 
@@ -106,9 +131,9 @@ class GradBucketReducer:
         if broadcast_params and self.world > 1:
             with torch.no_grad():
                 for p in params:
-                    dist.broadcast(p.data, 0, group=self.pg)
+                    broadcast(p.data, 0, group=self.pg)
                 for b in module.buffers():
-                    dist.broadcast(b, 0, group=self.pg)
+                    broadcast(b, 0, group=self.pg)
 
     def zero_grad(self):
         self.flat.zero_()
@@ -131,8 +156,9 @@ class GradBucketReducer:
             # where x/world == x*(1/world) exactly (powers of two)
             seg = self.flat[lo:hi]
             seg.mul_(self.inv_world)
-            h = dist.all_reduce(seg, op=dist.ReduceOp.SUM, group=self.pg, async_op=True)
-            self._handles.append((h, lo, hi))
+            h = all_reduce(seg, group=self.pg, async_op=True)
+            if h is not None:
+                self._handles.append((h, lo, hi))
 
     def _finish(self):
         for b in range(len(self.buckets)):

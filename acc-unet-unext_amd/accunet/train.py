@@ -38,6 +38,7 @@ import torch.distributed as dist
 import contextlib
 import os
 
+from . import dist as adist
 from . import kern, ops
 from . import profile as _prof
 from .loss import WeightedDiceBCE
@@ -191,9 +192,10 @@ class _GraphBuckets:
         main = torch.cuda.current_stream()
         narrow = self.wire is not self.flat
         if not nccl:  # gloo (tests): host-synchronous collectives on finished buckets
+            # the copies to the host run on this stream, behind the replay
             for k, (lo, hi) in enumerate(self.range):
                 self.events[k].synchronize()
-                dist.all_reduce(self.wire[lo:hi], op=dist.ReduceOp.SUM, group=pg)
+                adist.all_reduce(self.wire[lo:hi], group=pg)
                 if narrow:
                     self.flat[lo:hi].copy_(self.wire[lo:hi])
             return
@@ -251,7 +253,7 @@ class TrainStep:
             # identical replicas to start from (what DDP / GradBucketReducer do at wrap time)
             with torch.no_grad():
                 for t in list(self.params) + [b for b in model.buffers()]:
-                    dist.broadcast(t, 0, group=process_group)
+                    adist.broadcast(t, 0, group=process_group)
 
     def zero_grad(self):
         if self.reducer is not None:

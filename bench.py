@@ -502,7 +502,7 @@ def main():
     if world > 1:
         tt = torch.zeros(world, dtype=torch.float64, device=dev)
         tt[rank] = dt
-        dist.all_reduce(tt, op=dist.ReduceOp.SUM)  # every rank's time, in rank order
+        adist.all_reduce(tt)  # every rank's time, in rank order
         per_rank = tt.tolist()
         dt = max(per_rank)
     imgs = B * world * args.steps

@@ -16,12 +16,12 @@ def pytest_configure(config):
 
 # More than two gloo ranks on one GPU: test_world4 stopped without a word (180 s, no rank had
 # failed, the GPU still answered) while its ranks exchanged device tensors over gloo, which
-# is known to hang when several ranks share a card. Until those exchanges go through host
-# memory (accunet/dist.py, accunet/train.py, tests/dist_worker.py) these stay off the GPU; the
-# same exchanges run at world size 2 on the GPU and on CPU tensors in test_host_cpu.py.
+# is known to hang when several ranks share a card. The framework's collectives go through host
+# memory under gloo now (accunet/dist.py); dist_worker.py's own all_gather does not, so these
+# two stay off the GPU. test_gloo_host.py runs the same worker at world 2, 4 and 8 with that
+# call through host memory too.
 GLOO_ON_ONE_GPU = ("test_world4_buckets_and_wire_against_fp64_mean",
-                   "test_world8_buckets_and_wire_against_fp64_mean",
-                   "test_bench_gpus4_gloo_reports_four_ranks")
+                   "test_world8_buckets_and_wire_against_fp64_mean")
 
 
 # test_distill.py::test_hard_rows expects a wrong loss of its row 4, which lists one class many
