@@ -16,7 +16,7 @@ fi
 if [ "${ABI_HEADER:-}" = WORKTREE ]; then cp include/accunet.h _ab/${NAME}_src/include/accunet.h; fi
 ABI=0x$(sha256sum _ab/${NAME}_src/include/accunet.h | cut -c1-15)
 cd _ab/${NAME}_src/acc-unet-unext_amd/csrc
-ls *.hip | xargs -P 8 -I{} sh -c "/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result ${EXTRA_FLAGS:-} -DACCUNET_ABI_HASH=${ABI}LL -I../../include -I. -c {} -o {}.o"
+ls *.hip | xargs -P 8 -I{} sh -c "/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops ${EXTRA_FLAGS:-} -DACCUNET_ABI_HASH=${ABI}LL -I../../include -I. -c {} -o {}.o"
 /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -shared *.o -o ../../../$NAME/libaccunet_hip.so
 cd ../../.. && rm -rf ${NAME}_src
 ls -la $NAME

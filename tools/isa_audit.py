@@ -25,6 +25,7 @@ def compile_all(out, only):
         if only and not any(o in base for o in only):
             continue
         cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "--offload-device-only",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-S", "-I", os.path.join(ROOT, "include"), "-I", CSRC, src,
                "-o", os.path.join(out, base + ".s")]
         procs.append(subprocess.Popen(cmd, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL))

@@ -1,7 +1,7 @@
 // K1 access-shape lab: streaming kernels with the geometry of the HANC depthwise
 // forward (16x256x256x96 fp32 NHWC, 402 MB in + 402 MB out), no arithmetic, to find
 // which part of K1's structure costs bandwidth against a flat copy.
-//   hipcc -O3 --offload-arch=gfx950 tools/k1lab.hip -o tools/k1lab && tools/k1lab
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/k1lab.hip -o tools/k1lab && tools/k1lab
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>
