@@ -15,7 +15,7 @@
 // read and one write). Per-channel sums and parameters take 56 registers a thread, so a
 // row's threads are few enough for 2-3 waves a SIMD and the next row's loads are issued a
 // row ahead (327 -> 245 us at 16384 x 4096 bf16; parameters read 16 bytes at a time 194 us;
-// one block a CU and streaming stores 171 us, 4.7 TB/s).
+// one block a CU and streaming stores 171 us; 153-163 us, 4.9-5.3 TB/s, in later traces).
 #include "blocknorm.h"
 
 // ge: the gate has a row of its own for every token

@@ -281,7 +281,8 @@ ACC_DEV void dt_small_loss(const DtArgs& a, double* red) {
 
 // short rows: one wave a row, NQ vectors a lane in registers. The exponentials are relative
 // to the largest streamed class, which is the gradient's reference too (mu), so each is
-// computed once: dz = e * cu. 65536 x 2000 bf16 with 8 entries: 224 us in all.
+// computed once: dz = e * cu. 65536 x 2000 bf16 with 8 entries: 141-144
+// us of 203 for the whole pass.
 template <typename T, bool REST, int NQ>
 __global__ void __launch_bounds__(256)
 distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
@@ -370,7 +371,7 @@ distill_rows_wave_kernel(const DtArgs a, const DtScale g) {
 // without waiting for it.
 // The gradient's second read of the row misses the L2 but not the last-level cache (4096 x
 // 128000 bf16: 1.05 GB fetched from memory, 1.06 GB written), so two reads and a write cross
-// the fabric: 3.15 GB in 486-518 us, 6.1-6.5 TB/s, what a copy reaches. Loads a step ahead
+// the fabric: 3.15 GB in 476-518 us, 6.1-6.6 TB/s, what a copy reaches. Loads a step ahead
 // (488-571 us) or the row from its end changed nothing. Held in registers instead (64 a
 // thread for the row, one block a CU) it took 592-860 us: sums, barriers and stores of one
 // row then stand one behind another on each CU.

@@ -1,5 +1,5 @@
 // The 8-bit linear layer's product: C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]) over two
-// quantised matrices contracted along their rows (formats in fp8.h), fp32 accumulators.
+// quantised matrices contracted along their rows (formats in fp8.h).
 //
 // Two forms of the inner product:
 //   bf16 outputs: v_mfma_scale_f32_16x16x128_f8f6f4 contracts one 128-block of 16 rows of
@@ -76,9 +76,10 @@ ACC_DEV void fp8_store4(T* p, const float (&v)[4], int n, bool vec) {
 // WM x WN waves, TM x TN fragments of 16 x 16 each. 128 x 128 tiles (2 x 2 waves of 4 x 4)
 // read 64 KB of fragments a k-tile from LDS for 512 cycles of matrix work, which is more than
 // LDS delivers beside the copies; 256 x 256 tiles (2 x 4 waves of 8 x 4) read 192 KB for
-// 2048 cycles, one block a CU. 16384 x 4096 x 4096 in bf16: 272 us (2.02 PFLOP/s) with
-// 128 x 128, 242 us (2.27) with 256 x 256; fp32 outputs 485 and 422 us (1.30); 4096 x 4096 x
-// 16384 211 us (2.60).
+// 2048 cycles, one block a CU. Kernel traces on two cards, medians, normal data, with
+// 128 x 128 and 256 x 256: 16384 x 4096 x 4096 bf16 318-325 and 288-295 us (1.9 PFLOP/s), fp32
+// outputs 505-529 and 440-463 us (1.2); bf16 4096 x 4096 x 16384 254-264 and 213-234 us
+// (2.3-2.6), 4096 x 8192 x 8192 255-267 and 221-238 us (2.3-2.5).
 template <typename T, bool SPLIT, bool WIDE, int WM, int WN, int TM, int TN>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 fp8_gemm_kernel(const Fp8GemmArgs g) {
