@@ -65,8 +65,9 @@ def _apply(*args):
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, w1, b1, s, g, w2, b2, layer, eps, want_h, keep):
+        pre = "pre_" if f is not None else ""  # norm() has one weight and one bias
         P, L, C = _check(x, f, (("post_weight", w1), ("post_bias", b1), ("scale", s),
-                                ("pre_weight", w2), ("pre_bias", b2)), g)
+                                (pre + "weight", w2), (pre + "bias", b2)), g)
         r = torch.empty_like(x) if f is not None else None
         h = torch.empty_like(x) if want_h else None
         stats = torch.empty(P, 4, dtype=torch.float32, device=x.device) if keep else None
